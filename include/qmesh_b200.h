@@ -41,7 +41,8 @@ enum {
   QX_DEV_BAD_ID = 1,       /* an id outside {-1} U [0, E): that slot was skipped */
   QX_DEV_TIMEOUT = 2,      /* a bounded device wait ran out; the output is invalid */
   QX_DEV_OVERFLOW = 4,     /* more routed pairs than the workspace was sized for */
-  QX_DEV_NONFINITE = 8     /* qx_quant_fp8: a non-finite maximum; those bytes were not written */
+  QX_DEV_NONFINITE = 8     /* qx_quant_fp8: a non-finite maximum; those bytes were not written
+                              (qx_quant_int8: a row with a NaN or infinity; its scale is NaN) */
 };
 
 /* Activation formats. */
@@ -280,6 +281,57 @@ int qx_slice_decode_tc_xchg(const QxArena* arena, const QxSliceArgs* args, const
  * qx_slice_decode_tc (qx_slice_workspace_tc_bytes has room for it). */
 int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* args, const QxArena* shared,
                               const QxXchgArgs* x, void* stream);
+
+/* ---- 8-bit integer products (W8A8) --------------------------------------------
+ * Dense layers around the routed experts (the shared expert, projections) with
+ * int8 weights, one FP32 scale per output channel, and int8 activations, one
+ * FP32 scale per token. No counterpart in the reference.
+ *
+ * qx_quant_int8: x [rows, k] of type x_type (row stride x_stride elements) ->
+ * q[r, i] = round_half_even(127 x[r, i] / m_r), scale[r] = m_r / 127 with
+ * m_r = max(max_i |x[r, i]|, 1e-30). The quotient is rounded exactly for BF16,
+ * FP16 and E4M3 inputs; for FP32 after 127 x has been rounded to FP32. QX_T_E4M3:
+ * x = bf16(float(e4m3) x_scale), x_scale one value (n_scale = 1) or one per row
+ * (n_scale = rows), as the slice reads it. A row that holds a NaN or an infinity
+ * gets q = 0 and scale = NaN (every product with it is NaN; the other rows are
+ * not touched by it) and sets QX_DEV_NONFINITE (qx_int8_status). Weights are
+ * quantised with the same call, one scale per row of w [n, k]. rows = 0 does nothing.
+ *
+ * qx_int8_matmul: out[i, j] = ((float)(sum_k a[i, k] w[j, k]) * a_scale[i]) * w_scale[j],
+ * the sum exact in 32 bits, the result rounded once to out_type. With swiglu = 1,
+ * w holds n gate rows and then n up rows (w_scale too) and out[i, j] =
+ * g / (1 + exp(-g)) * u, with g = min(g, limit) and u = clamp(u, -limit, limit)
+ * first if has_limit. Strides in elements. The same bytes come out whatever m and
+ * the alignment are; rows of a and w that start on 16-byte boundaries (address
+ * and stride) run on the tensor cores, others on a slower path. m = 0 does
+ * nothing; out must not overlap the inputs.
+ *
+ * qx_int8_status: the QX_DEV_* bits (QX_DEV_NONFINITE, QX_DEV_TIMEOUT) that these
+ * calls recorded on the current device since the last read; reads, clears and
+ * waits for `stream`. */
+enum { QX_T_BF16 = 0, QX_T_F16 = 1, QX_T_F32 = 2, QX_T_E4M3 = 3 };
+#define QX_INT8_MAX_K 131071
+
+typedef struct {
+  const int8_t* a;         /* [m, k] activations */
+  int64_t       a_stride;
+  const float*  a_scale;   /* [m] */
+  const int8_t* w;         /* [n, k] weights ([2n, k] with swiglu) */
+  int64_t       w_stride;
+  const float*  w_scale;   /* [n] ([2n] with swiglu) */
+  void*         out;       /* [m, n] of out_type */
+  int64_t       out_stride;
+  int32_t       out_type;  /* QX_T_BF16, QX_T_F16 or QX_T_F32 */
+  int32_t       m, n, k;
+  int32_t       swiglu;
+  int32_t       has_limit;
+  float         limit;
+} QxInt8Args;
+
+int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* x_scale, int32_t n_scale,
+                  int64_t rows, int32_t k, int8_t* q, int64_t q_stride, float* scale, void* stream);
+int qx_int8_matmul(const QxInt8Args* args, void* stream);
+int qx_int8_status(uint32_t* status, void* stream);
 
 /* Self-check of the block-scaled NVFP4 tensor-core path (no counterpart in the
  * reference): d[128][n] (FP32, row-major) = sum over nkb 64-wide K blocks of

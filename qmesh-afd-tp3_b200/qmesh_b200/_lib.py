@@ -33,6 +33,7 @@ ERR_NAMES = {
 QX_DEV_BAD_ID = 1
 QX_DEV_TIMEOUT = 2
 QX_DEV_OVERFLOW = 4
+QX_DEV_NONFINITE = 8
 
 QX_LAYOUT_TC = 0x54430001
 QX_LAYOUT_FRAG = 0x46520002
@@ -40,6 +41,12 @@ QX_LAYOUT_FRAG = 0x46520002
 QX_X_E4M3 = 0
 QX_X_E4M3_POST = 1
 QX_X_BF16 = 2
+
+QX_T_BF16 = 0
+QX_T_F16 = 1
+QX_T_F32 = 2
+QX_T_E4M3 = 3
+INT8_MAX_K = 131071
 
 HIDDEN = 5120
 MAX_ROWS = 64
@@ -107,6 +114,26 @@ class QxXchgArgs(ctypes.Structure):
     ]
 
 
+class QxInt8Args(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("a_stride", ctypes.c_int64),
+        ("a_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_stride", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("out_type", ctypes.c_int32),
+        ("m", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("swiglu", ctypes.c_int32),
+        ("has_limit", ctypes.c_int32),
+        ("limit", ctypes.c_float),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point in include/qmesh_b200.h
 SIGNATURES = [
     ("qx_arena_w13_bytes", ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
@@ -155,6 +182,11 @@ SIGNATURES = [
     ("qx_slice_decode_tc_shared", ctypes.c_int,
      [ctypes.POINTER(QxArena), ctypes.POINTER(QxSliceArgs), ctypes.POINTER(QxArena), ctypes.POINTER(QxXchgArgs),
       ctypes.c_void_p]),
+    ("qx_quant_int8", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
+      ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    ("qx_int8_matmul", ctypes.c_int, [ctypes.POINTER(QxInt8Args), ctypes.c_void_p]),
+    ("qx_int8_status", ctypes.c_int, [ctypes.POINTER(ctypes.c_uint32), ctypes.c_void_p]),
     ("qx_combine_p2p", ctypes.c_int, [ctypes.POINTER(QxXchgArgs), ctypes.c_void_p]),
     ("qx_version", ctypes.c_char_p, []),
 ]

@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include "qmesh_b200.h"
 #include "qx_ptx.cuh"
@@ -218,13 +219,116 @@ __global__ void __launch_bounds__(256) plain_kernel(Args p) {
 }  // namespace i8
 }  // namespace qx
 
+#include "qx_int8_tc.cuh"
+
 using namespace qx::i8;
 
 namespace {
-bool on_b200() {
-  int dev = 0, major = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 &&
-         cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) == cudaSuccess && major == 10;
+// SMs of the current device, with the kernels' shared memory set up; 0 if it is no sm_100.
+int device_sms() {
+  static int cached[64] = {0};
+  int dev = 0, major = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (cached[dev]) return cached[dev];
+  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10) return 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaFuncSetAttribute(split_kernel<16>, attr, (int)Split<16>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(split_kernel<32>, attr, (int)Split<32>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(split_kernel<64>, attr, (int)Split<64>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(split_kernel<128>, attr, (int)Split<128>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(pair_kernel<128>, attr, (int)Pair<128>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(pair_kernel<256>, attr, (int)Pair<256>::SMEM) != cudaSuccess)
+    return 0;
+  return cached[dev] = sms;
+}
+
+uint64_t wait_limit_ns() {
+  const char* e = getenv("QX_TIMEOUT_MS");
+  const long ms = e ? atol(e) : 1000;
+  return (uint64_t)(ms < 10 ? 10 : ms) * 1000000ull;
+}
+
+// Tiled-copy descriptor of int8 rows [rows, k], boxes of 128 bytes x box_rows with
+// the 128-byte swizzle; places outside the tensor read as 0.
+bool row_map(CUtensorMap* map, const int8_t* base, int64_t rows, int k, int64_t stride, int box_rows) {
+  static decltype(&cuTensorMapEncodeTiled) encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &res) != cudaSuccess ||
+        res != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {KST, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, one,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN>
+int split_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int pieces, cudaStream_t st) {
+  const int half = p.swiglu ? 64 : 128;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = pieces;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.n + half - 1) / half * pieces), (unsigned)((p.m + BN - 1) / BN), 1);
+  cfg.blockDim = dim3(SPLIT_THR, 1, 1);
+  cfg.dynamicSmemBytes = Split<BN>::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, split_kernel<BN>, tw, ta, p, pieces, wait_limit_ns()) == cudaSuccess
+             ? QX_OK : QX_ERR_LAUNCH;
+}
+
+template <int BN>
+int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int sms, cudaStream_t st) {
+  const int cols = p.swiglu ? BN / 2 : BN;
+  const int tiles_m = (p.m + 255) / 256;
+  const int64_t tiles = (int64_t)tiles_m * ((p.n + cols - 1) / cols);
+  if (tiles > 0x7fffffff) return QX_ERR_SHAPE;
+  const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+  pair_kernel<BN><<<2 * pairs, PAIR_THR, Pair<BN>::SMEM, st>>>(tw, ta, p, tiles_m, (int)tiles, wait_limit_ns());
+  return cudaGetLastError() == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
+}
+
+// K pieces of the split kernel: the count (1..8) that leaves the busiest SM the
+// fewest K chunks, the smallest of equals.
+int pieces_of(int tiles, int chunks, int sms) {
+  int best = 1;
+  int64_t least = -1;
+  for (int s = 1; s <= 8 && s <= chunks; ++s) {
+    const int64_t c = (int64_t)((int64_t)tiles * s + sms - 1) / sms * ((chunks + s - 1) / s);
+    if (least < 0 || c < least) best = s, least = c;
+  }
+  return best;
+}
+
+int tc_launch(const Args& p, int sms, cudaStream_t st) {
+  CUtensorMap tw, ta;
+  const int64_t w_rows = p.swiglu ? 2ll * p.n : p.n;
+  if (p.m <= 128) {
+    const int bn = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+    if (!row_map(&tw, p.w, w_rows, p.k, p.ws, 64) || !row_map(&ta, p.a, p.m, p.k, p.as, bn)) return QX_ERR_DEVICE;
+    const int half = p.swiglu ? 64 : 128;
+    const int s = pieces_of((p.n + half - 1) / half, (p.k + (int)KST - 1) / (int)KST, sms);
+    return bn == 16 ? split_launch<16>(p, tw, ta, s, st) : bn == 32 ? split_launch<32>(p, tw, ta, s, st)
+         : bn == 64 ? split_launch<64>(p, tw, ta, s, st) : split_launch<128>(p, tw, ta, s, st);
+  }
+  // 256 or 128 weight rows per tile: whichever leaves the busiest pair fewer of them
+  const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, h = p.swiglu ? 2 : 1;
+  auto waves = [&](int bn) {
+    const int64_t t = (int64_t)tiles_m * ((p.n * (int64_t)h + bn - 1) / bn);
+    return (t + pairs - 1) / pairs * bn;
+  };
+  const int bn = waves(128) < waves(256) ? 128 : 256;
+  if (!row_map(&tw, p.w, w_rows, p.k, p.ws, bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, 128)) return QX_ERR_DEVICE;
+  return bn == 128 ? pair_launch<128>(p, tw, ta, sms, st) : pair_launch<256>(p, tw, ta, sms, st);
 }
 
 template <int T>
@@ -247,7 +351,7 @@ int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* 
   if (x_stride < k || q_stride < k) return QX_ERR_SHAPE;
   const int esz = x_type == QX_T_F32 ? 4 : x_type == QX_T_E4M3 ? 1 : 2;
   if (reinterpret_cast<uintptr_t>(x) % esz || reinterpret_cast<uintptr_t>(scale) % 4) return QX_ERR_ALIGN;
-  if (!on_b200()) return QX_ERR_DEVICE;
+  if (device_sms() <= 0) return QX_ERR_DEVICE;
   // four elements per access where every row starts on that boundary and has a multiple of four
   const bool vec = k % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * esz) == 0 && x_stride % 4 == 0 &&
                    reinterpret_cast<uintptr_t>(q) % 4 == 0 && q_stride % 4 == 0;
@@ -272,13 +376,23 @@ int qx_int8_matmul(const QxInt8Args* a, void* stream) {
   if (reinterpret_cast<uintptr_t>(a->out) % osz || reinterpret_cast<uintptr_t>(a->a_scale) % 4 ||
       reinterpret_cast<uintptr_t>(a->w_scale) % 4)
     return QX_ERR_ALIGN;
-  if (!on_b200()) return QX_ERR_DEVICE;
+  const int sms = device_sms();
+  if (sms <= 0) return QX_ERR_DEVICE;
   Args p;
   p.a = a->a; p.w = a->w; p.sa = a->a_scale; p.sw = a->w_scale; p.out = a->out;
   p.as = a->a_stride; p.ws = a->w_stride; p.os = a->out_stride;
   p.m = a->m; p.n = a->n; p.k = a->k; p.type = a->out_type;
   p.swiglu = a->swiglu ? 1 : 0; p.has_limit = a->has_limit ? 1 : 0; p.limit = a->limit;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // Tiled copies need rows that start on 16-byte boundaries (a single row: its address only).
+  auto aligned = [](const int8_t* b, int64_t stride, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(b) % 16 == 0 && (stride % 16 == 0 || rows == 1);
+  };
+  if (aligned(p.a, p.as, p.m) && aligned(p.w, p.ws, p.swiglu ? 2 : p.n)) {
+    if (p.m == 1) p.as = (p.as + 15) / 16 * 16;          // never stepped
+    if (p.n == 1 && !p.swiglu) p.ws = (p.ws + 15) / 16 * 16;
+    return tc_launch(p, sms, st);
+  }
   const int half = p.swiglu ? ST / 2 : ST;
   const int64_t gy = (p.m + ST - 1) / ST;
   if (gy > 65535) return QX_ERR_SHAPE;

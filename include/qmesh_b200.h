@@ -52,6 +52,9 @@ enum {
   QX_X_BF16 = 2    /* bf16 [rows, hidden] (the reference body's input) */
 };
 
+/* Element types of the calls that take several. */
+enum { QX_T_BF16 = 0, QX_T_F16 = 1, QX_T_F32 = 2, QX_T_E4M3 = 3 };
+
 /* Arena layouts: which kernel family the tiles were stored for. The two
  * layouts have the same byte counts, so the tag is the only thing that tells
  * them apart; every slice entry point refuses an arena whose tag is not its own
@@ -282,6 +285,40 @@ int qx_slice_decode_tc_xchg(const QxArena* arena, const QxSliceArgs* args, const
 int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* args, const QxArena* shared,
                               const QxXchgArgs* x, void* stream);
 
+/* ---- a whole MoE layer for a few tokens ----------------------------------------
+ * The router's product in front of the tensor-core slice, as two kernels (the
+ * reference takes ids and weights from its serving engine's router,
+ * afd_session.py:211-252; no counterpart there):
+ *   l[r, e] = sum_k x[r, k] gate[e, k] (+ bias[e])          FP32 sums
+ *   ids[r]  = the topk experts of the largest l (larger first, lower id first
+ *             among equals; a NaN counts as the largest; an expert whose l is
+ *             -infinity is not selected: its slot gets id -1 and weight 0)
+ *   tw[r,j] = exp(l_j - l_0) / sum_i exp(l_i - l_0) over the selected slots
+ *   out[r]  = bf16(sum_j tw_j E_{ids_j}(x_r) [+ S(x_r)] [+ addend[r]]), summed in
+ *             FP32 in that order and rounded once
+ * with E and S the NVFP4 SwiGLU experts of qx_slice_decode_tc over the arena's
+ * columns [c0, c1) and of the one-expert arena `shared` (or NULL). args as for
+ * qx_slice_decode_tc, except that ids, ids_int64 and tw are not read and the
+ * workspace has qx_moe_workspace_bytes bytes (0 for sizes the call refuses:
+ * 1..QX_MAX_ROWS rows, topk 1..min(QX_MAX_TOPK, n_experts), n_experts up to 4096).
+ * A row whose logits hold a NaN or +infinity has NaN weights and a NaN output;
+ * the other rows are as without it. Capture-safe; calls that may overlap on the
+ * GPU need a workspace each. */
+typedef struct {
+  const void*  gate;         /* router weights [n_experts, 5120], 16-byte aligned rows */
+  int32_t      gate_type;    /* QX_T_BF16 or QX_T_F32 */
+  int64_t      gate_stride;  /* elements between rows */
+  const float* bias;         /* [n_experts] added to the logits, or NULL */
+  int32_t*     ids;          /* optional outputs [rows, topk], or NULL */
+  float*       tw;
+  const float* addend;       /* optional FP32 [rows, 5120] (a shared expert computed elsewhere), or NULL */
+  int64_t      addend_stride;
+} QxRouterArgs;
+
+size_t qx_moe_workspace_bytes(int32_t rows, int32_t n_experts, int32_t topk, int32_t c0, int32_t c1);
+int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRouterArgs* router, const QxArena* shared,
+                     void* stream);
+
 /* ---- 8-bit integer products (W8A8) --------------------------------------------
  * Dense layers around the routed experts (the shared expert, projections) with
  * int8 weights, one FP32 scale per output channel, and int8 activations, one
@@ -309,7 +346,6 @@ int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* args, con
  * qx_int8_status: the QX_DEV_* bits (QX_DEV_NONFINITE, QX_DEV_TIMEOUT) that these
  * calls recorded on the current device since the last read; reads, clears and
  * waits for `stream`. */
-enum { QX_T_BF16 = 0, QX_T_F16 = 1, QX_T_F32 = 2, QX_T_E4M3 = 3 };
 #define QX_INT8_MAX_K 131071
 
 typedef struct {

@@ -56,9 +56,15 @@
 //                      of y_j) [+ the shared expert's bf16 output], once their
 //                      tile's counter is complete, or hands them to the fused rank
 //                      combine (qx_xchg.cuh).
+//
+// A whole MoE layer (qx_moe_decode_tc) is the same pair with the router in
+// front: moe_front_kernel computes the router's logits beside the x terms, and
+// every CTA of tc_decode_kernel<true> selects the top-k from them itself before
+// it builds the routing tables, so the layer is two kernels.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
+#include <math.h>
 #include <stdint.h>
 #include <stdlib.h>
 
@@ -206,6 +212,16 @@ struct Params {
   const __nv_bfloat16* xshared;
   int64_t xshared_stride;
   int xrank, xworld, xdst, xrows_max;
+  // whole MoE layer (qx_moe_decode_tc): ids and tw are selected from the logits
+  float* logits;          // [rows][E], written by moe_front_kernel
+  const void* gate;       // router weights [E][HID], BF16 or FP32, rows gate_stride elements apart
+  int64_t gate_stride;
+  const float* gate_bias; // [E] or null
+  int32_t* ids_out;       // optional outputs [rows, topk]
+  float* tw_out;
+  const float* addend;    // optional FP32 [rows][HID] added before the output's rounding
+  int64_t addend_stride;
+  int sel_off;            // shared-memory offset of the selected ids [P], then weights [P]
 };
 
 struct ItemMeta {
@@ -364,12 +380,15 @@ constexpr int IDR = MAXP / 32;   // expert ids per lane of the routing warp
 
 // Lane `lane`'s expert ids (pairs lane + 32 i); ids outside [0, E) (the -1
 // sentinel, or bad ids that the prep kernel flags) become -1 and are skipped.
-__device__ __forceinline__ void load_ids(const Params& p, int lane, int (&idr)[IDR]) {
+// `sel`: the ids selected in this CTA's shared memory (a whole MoE layer), or null.
+__device__ __forceinline__ void load_ids(const Params& p, const int32_t* sel, int lane, int (&idr)[IDR]) {
 #pragma unroll
   for (int i = 0; i < IDR; ++i) {
     const int q = lane + 32 * i;
     long long id = -1;
-    if (q < p.P)
+    if (q < p.P && sel)
+      id = sel[q];
+    else if (q < p.P)
       id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + q)
                    : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + q);
     idr[i] = (id >= 0 && id < p.E) ? (int)id : -1;
@@ -642,14 +661,14 @@ __device__ void route_local(const Params& p, const int (&idr)[IDR], GroupS* gs, 
 // row computes the same), and the chunk's 16 unscaled x terms
 // q_t = rne(r_t / 2^(E - 2t)) (two elements per thread) into the row's stage
 // block. CTA 0 also resets the call's counters and records bad ids.
-__global__ void __launch_bounds__(PREP_THR) tc_prep_kernel(Params p) {
+// `units`: CTAs that run it; `given`: the call's ids are an input (to be checked).
+__device__ __forceinline__ void prep_unit(const Params& p, int units, bool given) {
   __shared__ float red[PREP_THR / 32];
-  pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31;
   if (blockIdx.x == 0) {
     bool bad = false;
     for (int q = tid; q < p.P + p.rows; q += PREP_THR) {
-      if (q < p.P) {
+      if (given && q < p.P) {
         const long long id = p.ids64 ? reinterpret_cast<const long long*>(p.ids)[q]
                                      : (long long)reinterpret_cast<const int*>(p.ids)[q];
         bad |= !(id == -1 || (id >= 0 && id < p.E));
@@ -665,7 +684,7 @@ __global__ void __launch_bounds__(PREP_THR) tc_prep_kernel(Params p) {
     __syncthreads();
     if (tid == 0 && bad) p.ctl->status = (uint32_t)QX_DEV_BAD_ID;
   }
-  for (int i = blockIdx.x * PREP_THR + tid; i < MAXSPLIT + MAXSG * MAX_STILES; i += gridDim.x * PREP_THR)
+  for (int i = blockIdx.x * PREP_THR + tid; i < MAXSPLIT + MAXSG * MAX_STILES; i += units * PREP_THR)
     p.pcnt[i] = 0;
   const int r = blockIdx.x / NXCH, c = blockIdx.x - r * NXCH;
   float inv = 1.f;
@@ -688,6 +707,13 @@ __global__ void __launch_bounds__(PREP_THR) tc_prep_kernel(Params p) {
     ig *= 4.f;
   }
 }
+
+__global__ void __launch_bounds__(PREP_THR) tc_prep_kernel(Params p) {
+  pdl_launch_dependents();
+  prep_unit(p, gridDim.x, true);
+}
+
+#include "qx_router.cuh"
 
 __device__ __forceinline__ void st_release_gpu(uint32_t* ptr, uint32_t v) {
   asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(ptr), "r"(v) : "memory");
@@ -988,10 +1014,13 @@ __device__ __forceinline__ bool second_acc(const ItemMeta& m) { return m.nst > 1
 // row 4 rb + et / 32: bf16(sum over slots j in order of y[row * topk + j][k]),
 // a slot without a valid expert adding 0. Returns the 4 BF16 values (zeros for a
 // row past the post's last).
-__device__ uint2 unit_partial(const Params& p, int tile, int rb, int et, int& row, int& k) {
+// `sel`: the call's ids in shared memory, or null (as load_ids). unit_sum is the
+// FP32 sum before the rounding.
+__device__ __forceinline__ float4 unit_sum(const Params& p, const int32_t* sel, int tile, int rb, int et, int& row,
+                                           int& k) {
   k = tile * 128 + 4 * (et & 31);
   row = 4 * rb + (et >> 5);
-  if (row >= p.rows) return make_uint2(0u, 0u);
+  if (row >= p.rows) return make_float4(0.f, 0.f, 0.f, 0.f);
   float4 v[QX_MAX_TOPK];
   bool val[QX_MAX_TOPK];
 #pragma unroll
@@ -1000,8 +1029,9 @@ __device__ uint2 unit_partial(const Params& p, int tile, int rb, int et, int& ro
     v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (j < p.topk) {
       const int q = row * p.topk + j;
-      const long long id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + q)
-                                   : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + q);
+      const long long id = sel ? (long long)sel[q]
+                           : p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + q)
+                                     : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + q);
       val[j] = id >= 0 && id < p.E;
       v[j] = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)q * HID + k));
     }
@@ -1015,6 +1045,11 @@ __device__ uint2 unit_partial(const Params& p, int tile, int rb, int et, int& ro
     s.z += z.z;
     s.w += z.w;
   }
+  return s;
+}
+
+__device__ uint2 unit_partial(const Params& p, int tile, int rb, int et, int& row, int& k) {
+  const float4 s = unit_sum(p, nullptr, tile, rb, et, row, k);
   const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
@@ -1137,11 +1172,32 @@ __device__ bool finalize_unit(const Params& p, Smem& S, int u, int tile, int rb,
   return true;
 }
 
+// Finalize unit of a whole MoE layer on one GPU: the routed sum, the shared
+// expert's FP32 output and the addend meet in FP32 and are rounded once (no
+// transport of BF16 partials lies between them here).
+__device__ void finalize_moe(const Params& p, const int32_t* sel, int tile, int rb, int et) {
+  int row, k;
+  float4 s = unit_sum(p, sel, tile, rb, et, row, k);
+  if (row >= p.rows) return;
+  if (p.sNT > 0) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)(p.P + row) * HID + k));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  if (p.addend) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p.addend + (size_t)row * p.addend_stride + k));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const float o[4] = {s.x, s.y, s.z, s.w};
+  *reinterpret_cast<uint2*>(p.out + (size_t)row * p.out_stride + k) = pack_bf16x4(o);
+}
+
 // Epilogue warpgroup eg (warps 2-5 or 7-10): the items of accumulator buffer
 // eg, i.e. every other item. Named barriers 1 + 2 eg (its 128 threads) and
 // 2 + 2 eg (its gate half).
-__device__ void epilogue(const Params& p, Smem& S, float* xg, const GroupS* gs, const PairS* ps, uint32_t tbase,
-                         int eg, volatile uint32_t* status, uint64_t deadline) {
+// MOE: ids and weights are the ones selected in shared memory at `sel`.
+template <bool MOE>
+__device__ void epilogue(const Params& p, Smem& S, float* xg, const GroupS* gs, const PairS* ps, const int32_t* sel,
+                         uint32_t tbase, int eg, volatile uint32_t* status, uint64_t deadline) {
   xg += eg * 2 * p.gmax * 64;
   float* xu = xg + p.gmax * 64;                  // gate and up values of a gate/up item, [pair][column]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1181,7 +1237,8 @@ __device__ void epilogue(const Params& p, Smem& S, float* xg, const GroupS* gs, 
       g2c = __ldg(gr.shared ? p.sg2 : &p.g2[gr.expert]);
       if (et < gr.gsz) {
         const int pq = ps[gr.pair_off + et].pq;
-        tws[et] = pq < p.P ? __ldg(&p.tw[pq]) : 1.f;
+        if constexpr (MOE) tws[et] = pq < p.P ? reinterpret_cast<const float*>(sel + p.P)[pq] : 1.f;
+        else tws[et] = pq < p.P ? __ldg(&p.tw[pq]) : 1.f;
         if (p.ae_fixed) {
           em[et] = p.ae_val;           // every tile's exponent; the producer waited for the terms
         } else {
@@ -1373,10 +1430,12 @@ __device__ void epilogue(const Params& p, Smem& S, float* xg, const GroupS* gs, 
     bool ok = true;
     if (et == 0) ok = wait_flag(&p.fcnt[tile], (uint32_t)S.hdr.n_fin, status, deadline);
     if (!bar_and(B1, 128, ok)) break;   // every thread's y reads follow thread 0's acquire
-    if (!finalize_unit(p, S, u, tile, u - tile * rbn, et, eg, B1, const_cast<uint32_t*>(status), deadline)) break;
+    if constexpr (MOE) finalize_moe(p, sel, tile, u - tile * rbn, et);
+    else if (!finalize_unit(p, S, u, tile, u - tile * rbn, et, eg, B1, const_cast<uint32_t*>(status), deadline)) break;
   }
 }
 
+template <bool MOE>
 __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   Smem& S = *reinterpret_cast<Smem*>(smem);
@@ -1388,7 +1447,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   volatile uint32_t* status = &p.ctl->status;
   // Warp 0 loads the call's expert ids while other warps set up the CTA.
   int idr[IDR];
-  if (warp == 0) load_ids(p, threadIdx.x & 31, idr);
+  int32_t* sel = MOE ? reinterpret_cast<int32_t*>(smem + p.sel_off) : nullptr;
+  if (!MOE && warp == 0) load_ids(p, nullptr, threadIdx.x & 31, idr);
   if (threadIdx.x == 64) {
     for (int s = 0; s < MAXNS; ++s) {
       mbar_init(&S.full[s], 1);
@@ -1428,7 +1488,15 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     S.mma_scratch[0] = 0;
     mbar_wait_bounded(&S.init_bar, 0, &S.mma_scratch[0], 1u, globaltimer_ns() + p.timeout_ns);
   }
-  // The ids come from work before the prep kernel (which is launched without
+  if constexpr (MOE) {
+    // The logits are the front kernel's: wait for it, then select every row's
+    // experts (each CTA all rows, a warp per row; CTA 0 also writes them out).
+    pdl_wait();
+    select_rows(p, sel, reinterpret_cast<float*>(sel + p.P), warp, NTHR / 32);
+    __syncthreads();
+    if (warp == 0) load_ids(p, sel, threadIdx.x & 31, idr);
+  }
+  // Otherwise the ids come from work before the prep kernel (which is launched without
   // early start), so the routing needs no wait; the prep kernel's results are
   // waited for by the threads that read them (producer, epilogue).
   if (warp == 0) route_local(p, idr, gs, ps, &S.hdr);
@@ -1453,7 +1521,7 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   } else if (warp == 1 || warp == 6) {
     if ((threadIdx.x & 31) == 0) mma_issuer(p, ring, S, gs, tbase, warp == 1 ? 0 : 1, status, deadline);
   } else {
-    epilogue(p, S, xg, gs, ps, tbase, warp < 6 ? 0 : 1, status, deadline);
+    epilogue<MOE>(p, S, xg, gs, ps, sel, tbase, warp < 6 ? 0 : 1, status, deadline);
   }
   // The producer drained its copies and the issuers their tensor-core work (all
   // bounded) before returning; the epilogue's last TMEM reads are complete.
@@ -1489,8 +1557,10 @@ static int device_sms(int* dev_out) {
     cached[dev] = sms;
   }
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(tc_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(tc_decode_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)SMEM_LIMIT) != cudaSuccess ||
+        cudaFuncSetAttribute(tc_decode_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)SMEM_LIMIT) != cudaSuccess)
       return -1;
     attr_set[dev] = true;
   }
@@ -1535,14 +1605,20 @@ size_t qx_slice_workspace_tc_bytes(int32_t rows, int32_t topk, int32_t c0, int32
   return ws_layout(rows, topk, c1 - c0).total;
 }
 
+size_t qx_moe_workspace_bytes(int32_t rows, int32_t n_experts, int32_t topk, int32_t c0, int32_t c1) {
+  const size_t n = qx_slice_workspace_tc_bytes(rows, topk, c0, c1);
+  if (n == 0 || n_experts < 1 || n_experts > MAXE || topk > n_experts) return 0;
+  return n + (size_t)rows * n_experts * sizeof(float);   // the slice's, then the logits
+}
+
 }  // extern "C"
 
 // The slice call, alone (x == nullptr) or with the fused rank combine, and with
 // the shared expert's arena (sh) on the output rank.
 static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArgs* x, const QxArena* sh,
-                     void* stream) {
+                     void* stream, const QxRouterArgs* rt = nullptr) {
   if (!arena || !a) return QX_ERR_ARG;
-  if (!a->x || !a->ids || !a->tw || !a->out || !a->workspace || !arena->w13 || !arena->w2 || !arena->g13 ||
+  if (!a->x || (!rt && (!a->ids || !a->tw)) || !a->out || !a->workspace || !arena->w13 || !arena->w2 || !arena->g13 ||
       !arena->g2)
     return QX_ERR_ARG;
   if ((a->x_fmt == QX_X_E4M3 || a->x_fmt == QX_X_E4M3_POST) && !a->x_scale) return QX_ERR_ARG;
@@ -1564,6 +1640,19 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   const int W = a->c1 - a->c0;
   const WsLayout L = ws_layout(a->rows, a->topk, W);
   if (a->workspace_bytes < L.total) return QX_ERR_WORKSPACE;
+  if (rt) {
+    if (!rt->gate || (rt->gate_type != QX_T_BF16 && rt->gate_type != QX_T_F32)) return QX_ERR_ARG;
+    if (a->topk > arena->n_experts || rt->gate_stride < HID) return QX_ERR_SHAPE;
+    const int per16 = rt->gate_type == QX_T_BF16 ? 8 : 4;   // router weights per 16 bytes
+    if ((reinterpret_cast<uintptr_t>(rt->gate) & 15u) || rt->gate_stride % per16 ||
+        (reinterpret_cast<uintptr_t>(rt->bias) & 3u) || (reinterpret_cast<uintptr_t>(rt->ids) & 3u) ||
+        (reinterpret_cast<uintptr_t>(rt->tw) & 3u))
+      return QX_ERR_ALIGN;
+    if (rt->addend && rt->addend_stride < HID) return QX_ERR_SHAPE;
+    if (rt->addend && ((reinterpret_cast<uintptr_t>(rt->addend) & 15u) || rt->addend_stride % 4)) return QX_ERR_ALIGN;
+    if (a->workspace_bytes < qx_moe_workspace_bytes(a->rows, arena->n_experts, a->topk, a->c0, a->c1))
+      return QX_ERR_WORKSPACE;
+  }
   int dev = 0;
   const int sms = device_sms(&dev);
   if (sms <= 0) return QX_ERR_DEVICE;
@@ -1614,7 +1703,9 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   const size_t xchg = (size_t)NEPI * 2 * p.gmax * 64 * sizeof(float);
   p.x_off = (int)((sizeof(Smem) + 15) & ~size_t(15));
   p.tab_off = (int)(((size_t)p.x_off + xchg + 15) & ~size_t(15));
-  p.ring_off = (int)(((size_t)p.tab_off + tables + 127) & ~size_t(127));
+  p.sel_off = (int)((size_t)p.tab_off + tables);
+  const size_t sel = rt ? (size_t)p.P * (sizeof(int32_t) + sizeof(float)) : 0;
+  p.ring_off = (int)(((size_t)p.sel_off + sel + 127) & ~size_t(127));
   p.ring_bytes = (int)(SMEM_LIMIT - (size_t)p.ring_off);
   if (p.ring_bytes - 512 < 2 * (A_STAGE + p.bst)) return QX_ERR_SHAPE;   // two slots of the widest group
   p.ns = p.b_off = 0;
@@ -1675,10 +1766,29 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
     p.sW = sh->a1 - sh->a0;
     p.sNT = (p.sW + 63) / 64;
   }
+  p.logits = nullptr;
+  p.gate = nullptr;
+  p.gate_stride = p.addend_stride = 0;
+  p.gate_bias = p.addend = nullptr;
+  p.ids_out = nullptr;
+  p.tw_out = nullptr;
+  if (rt) {
+    p.ids = nullptr;
+    p.tw = nullptr;
+    p.logits = reinterpret_cast<float*>(ws + L.total);
+    p.gate = rt->gate;
+    p.gate_stride = rt->gate_stride;
+    p.gate_bias = rt->bias;
+    p.ids_out = rt->ids;
+    p.tw_out = rt->tw;
+    p.addend = rt->addend;
+    p.addend_stride = rt->addend_stride;
+  }
   const size_t smem_bytes = SMEM_LIMIT;
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  tc_prep_kernel<<<a->rows * NXCH, PREP_THR, 0, st>>>(p);
+  if (rt) front_launch(p, rt->gate_type, st);
+  else tc_prep_kernel<<<a->rows * NXCH, PREP_THR, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return QX_ERR_LAUNCH;
 
   cudaLaunchAttribute attr[1];
@@ -1691,8 +1801,9 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, tc_decode_kernel, p) != cudaSuccess) return QX_ERR_LAUNCH;
-  return QX_OK;
+  const cudaError_t err = rt ? cudaLaunchKernelEx(&cfg, tc_decode_kernel<true>, p)
+                             : cudaLaunchKernelEx(&cfg, tc_decode_kernel<false>, p);
+  return err == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
 }
 
 extern "C" {
@@ -1710,6 +1821,12 @@ int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* a, const 
                               const QxXchgArgs* x, void* stream) {
   if (!shared) return QX_ERR_ARG;
   return tc_launch(arena, a, x, shared, stream);
+}
+
+int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* a, const QxRouterArgs* router, const QxArena* shared,
+                     void* stream) {
+  if (!router) return QX_ERR_ARG;
+  return tc_launch(arena, a, nullptr, shared, stream, router);
 }
 
 }  // extern "C"

@@ -114,6 +114,19 @@ class QxXchgArgs(ctypes.Structure):
     ]
 
 
+class QxRouterArgs(ctypes.Structure):
+    _fields_ = [
+        ("gate", ctypes.c_void_p),
+        ("gate_type", ctypes.c_int32),
+        ("gate_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("ids", ctypes.c_void_p),
+        ("tw", ctypes.c_void_p),
+        ("addend", ctypes.c_void_p),
+        ("addend_stride", ctypes.c_int64),
+    ]
+
+
 class QxInt8Args(ctypes.Structure):
     _fields_ = [
         ("a", ctypes.c_void_p),
@@ -181,6 +194,11 @@ SIGNATURES = [
      [ctypes.POINTER(QxArena), ctypes.POINTER(QxSliceArgs), ctypes.POINTER(QxXchgArgs), ctypes.c_void_p]),
     ("qx_slice_decode_tc_shared", ctypes.c_int,
      [ctypes.POINTER(QxArena), ctypes.POINTER(QxSliceArgs), ctypes.POINTER(QxArena), ctypes.POINTER(QxXchgArgs),
+      ctypes.c_void_p]),
+    ("qx_moe_workspace_bytes", ctypes.c_size_t,
+     [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    ("qx_moe_decode_tc", ctypes.c_int,
+     [ctypes.POINTER(QxArena), ctypes.POINTER(QxSliceArgs), ctypes.POINTER(QxRouterArgs), ctypes.POINTER(QxArena),
       ctypes.c_void_p]),
     ("qx_quant_int8", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,

@@ -24,6 +24,8 @@ import torch
 
 from . import _lib
 from .arena import Arena
+from .combine import combine_ordered
+from .int8 import Int8Expert
 from .trace import rng
 
 SWIGLU_LIMIT = 10.0
@@ -47,7 +49,10 @@ def _ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
 
 
-def _slice_args(x, ids, tw, out, c0, c1, workspace, x_scale, swiglu_limit, has_limit) -> _lib.QxSliceArgs:
+def _slice_args(x, ids, tw, out, c0, c1, workspace, x_scale, swiglu_limit, has_limit,
+                topk: int | None = None) -> _lib.QxSliceArgs:
+    """Checked arguments of a slice call. With `topk`, ids and tw are not inputs (the
+    whole MoE layer selects them itself)."""
     rows = x.shape[0]
     if x.dtype == torch.bfloat16:
         fmt = _lib.QX_X_BF16
@@ -63,19 +68,24 @@ def _slice_args(x, ids, tw, out, c0, c1, workspace, x_scale, swiglu_limit, has_l
         esz = 1
     else:
         raise TypeError(f"x must be bf16 or e4m3, got {x.dtype}")
-    if ids.dtype not in (torch.int32, torch.int64) or tw.dtype != torch.float32 or out.dtype != torch.bfloat16:
+    if topk is not None:
+        if out.dtype != torch.bfloat16:
+            raise TypeError(f"out must be bf16, got {out.dtype}")
+        if out.dim() != 2 or out.shape[0] < rows:
+            raise ValueError(f"shape mismatch: x {tuple(x.shape)} out {tuple(out.shape)}")
+    elif ids.dtype not in (torch.int32, torch.int64) or tw.dtype != torch.float32 or out.dtype != torch.bfloat16:
         raise TypeError(f"ids/tw/out must be int32|int64/f32/bf16, got {ids.dtype}/{tw.dtype}/{out.dtype}")
-    if ids.shape != tw.shape or ids.shape[0] != rows or out.shape[0] < rows:
+    elif ids.shape != tw.shape or ids.shape[0] != rows or out.shape[0] < rows:
         raise ValueError(f"shape mismatch: x {tuple(x.shape)} ids {tuple(ids.shape)} tw {tuple(tw.shape)} "
                          f"out {tuple(out.shape)}")
     if x.shape[1] != _lib.HIDDEN or out.shape[1] != _lib.HIDDEN:
         raise ValueError(f"hidden size must be {_lib.HIDDEN}")
-    if not (ids.is_contiguous() and tw.is_contiguous()) or x.stride(1) != 1 or out.stride(1) != 1:
+    if (topk is None and not (ids.is_contiguous() and tw.is_contiguous())) or x.stride(1) != 1 or out.stride(1) != 1:
         raise ValueError("ids/tw must be contiguous and x/out rows unit-stride")
     return _lib.QxSliceArgs(
         _ptr(x), _ptr(x_scale), x.stride(0) * esz, fmt,
-        _ptr(ids), 1 if ids.dtype == torch.int64 else 0, _ptr(tw),
-        rows, ids.shape[1], c0, c1, float(swiglu_limit), 1 if has_limit else 0,
+        _ptr(ids), 1 if topk is None and ids.dtype == torch.int64 else 0, _ptr(tw),
+        rows, ids.shape[1] if topk is None else topk, c0, c1, float(swiglu_limit), 1 if has_limit else 0,
         _ptr(out), out.stride(0), _ptr(workspace), workspace.numel())
 
 
@@ -204,10 +214,14 @@ def launch_prefill(view: _lib.QxArena, x: torch.Tensor, ids: torch.Tensor, tw: t
 def prefill_slice(arena: Arena, li: int, x: torch.Tensor, ids: torch.Tensor, tw: torch.Tensor, a2: torch.Tensor,
                   c0: int | None = None, c1: int | None = None, x_scale: torch.Tensor | None = None,
                   out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
-                  swiglu_limit: float = SWIGLU_LIMIT) -> torch.Tensor:
-    """BF16 [rows, 5120] partial of a prefill chunk over columns [c0, c1) (W4A4)."""
+                  swiglu_limit: float = SWIGLU_LIMIT, shared: Int8Expert | None = None) -> torch.Tensor:
+    """BF16 [rows, 5120] partial of a prefill chunk over columns [c0, c1) (W4A4). With
+    `shared`, a W8A8 expert over the same rows is added after the routed partial in the
+    ordered combine's arithmetic, bf16(fp32(routed) + fp32(shared)), each part BF16."""
     if arena.layout != "tc":
         raise ValueError("the prefill slice needs a tensor-core layout arena")
+    if shared is not None and shared.k != _lib.HIDDEN:
+        raise ValueError(f"the shared expert's width is {shared.k}, the slice's {_lib.HIDDEN}")
     c0 = arena.a0 if c0 is None else c0
     c1 = arena.a1 if c1 is None else c1
     rows = x.shape[0]
@@ -215,8 +229,11 @@ def prefill_slice(arena: Arena, li: int, x: torch.Tensor, ids: torch.Tensor, tw:
         out = torch.empty(rows, _lib.HIDDEN, dtype=torch.bfloat16, device=x.device)
     if workspace is None:
         workspace = alloc_prefill_workspace(rows, ids.shape[1], c0, c1, arena.n_experts, x.device)
-    launch_prefill(arena.view(li), x, ids, tw, a2, out, c0, c1, workspace, x_scale=x_scale,
+    routed = out if shared is None else torch.empty(rows, _lib.HIDDEN, dtype=torch.bfloat16, device=x.device)
+    launch_prefill(arena.view(li), x, ids, tw, a2, routed, c0, c1, workspace, x_scale=x_scale,
                    swiglu_limit=max(swiglu_limit, 0.0), has_limit=swiglu_limit > 0)
+    if shared is not None:
+        combine_ordered([routed, shared(x, x_scale)], out=out[:rows])
     return out
 
 

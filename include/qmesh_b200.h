@@ -364,9 +364,40 @@ typedef struct {
   float         limit;
 } QxInt8Args;
 
-int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* x_scale, int32_t n_scale,
+int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* x_scale, int64_t n_scale,
                   int64_t rows, int32_t k, int8_t* q, int64_t q_stride, float* scale, void* stream);
 int qx_int8_matmul(const QxInt8Args* args, void* stream);
+
+/* A dense SwiGLU expert in 8 bits, the four calls as one: quantise x, the SwiGLU
+ * product with w13 [2 inter, k] into FP32, quantise that, the product with w2
+ * [k, inter] into out [rows, k]. The same bytes as the separate calls; workspace
+ * of qx_int8_expert_workspace_bytes, 16-byte aligned, not shared by calls that may
+ * overlap on the GPU. The weights must have been written by work that was queued
+ * on the stream (or completed) before this call. rows = 0 does nothing. */
+typedef struct {
+  const void*   x;         /* [rows, k] of x_type, as qx_quant_int8 */
+  int64_t       x_stride;
+  int32_t       x_type;
+  int32_t       n_scale;
+  const float*  x_scale;
+  const int8_t* w13;       /* gate rows, then up rows */
+  int64_t       w13_stride;
+  const float*  w13_scale; /* [2 inter] */
+  const int8_t* w2;
+  int64_t       w2_stride;
+  const float*  w2_scale;  /* [k] */
+  void*         out;       /* [rows, k] of out_type */
+  int64_t       out_stride;
+  int32_t       out_type;
+  int32_t       rows, k, inter;
+  int32_t       has_limit;
+  float         limit;
+  void*         workspace;
+  size_t        workspace_bytes;
+} QxInt8ExpertArgs;
+
+size_t qx_int8_expert_workspace_bytes(int32_t rows, int32_t k, int32_t inter);
+int qx_int8_expert(const QxInt8ExpertArgs* args, void* stream);
 int qx_int8_status(uint32_t* status, void* stream);
 
 /* Self-check of the block-scaled NVFP4 tensor-core path (no counterpart in the

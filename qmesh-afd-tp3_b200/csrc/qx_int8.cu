@@ -50,99 +50,159 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit, bool has_
 }
 
 // ------------------------------------------------------------------ quantiser
-// Four elements of a row from k on (k % 4 == 0; those past the row's end read as 0),
-// as FP32: BF16 / FP16 / FP32 values, or the slice's FP8 form bf16(float(e4m3) inv).
-template <int T, bool VEC>
-__device__ __forceinline__ void load4(const void* x, int64_t row_off, int k, int n, float inv, float (&v)[4]) {
-  if constexpr (T == QX_T_F32) {
-    const float* p = reinterpret_cast<const float*>(x) + row_off + k;
-    if (VEC) {
-      const float4 w = *reinterpret_cast<const float4*>(p);
-      v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+// Elements of type T per 16-byte load.
+template <int T>
+__host__ __device__ constexpr int per16() { return T == QX_T_F32 ? 4 : T == QX_T_E4M3 ? 16 : 8; }
+
+// The FP32 values of one 16-byte load: BF16 / FP16 / FP32 values, or the slice's
+// FP8 form bf16(float(e4m3) inv).
+template <int T>
+__device__ __forceinline__ void unpack(const uint4& raw, float inv, float (&v)[per16<T>()]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == QX_T_F32) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (T == QX_T_BF16) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else if constexpr (T == QX_T_F16) {
+      v[2 * i] = f16lo_to_f32(w[i]);
+      v[2 * i + 1] = f16hi_to_f32(w[i]);
     } else {
+      const uint32_t lo = e4m3x2_to_f16x2(w[i] & 0xffffu), hi = e4m3x2_to_f16x2(w[i] >> 16);
+      const float f[4] = {f16lo_to_f32(lo), f16hi_to_f32(lo), f16lo_to_f32(hi), f16hi_to_f32(hi)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = k + i < n ? p[i] : 0.f;
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = __bfloat162float(__float2bfloat16_rn(__fmul_rn(f[j], inv)));
     }
-  } else if constexpr (T == QX_T_E4M3) {
-    const uint8_t* p = reinterpret_cast<const uint8_t*>(x) + row_off + k;
-    uint32_t w = 0;
-    if (VEC) w = *reinterpret_cast<const uint32_t*>(p);
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w |= (k + i < n ? (uint32_t)p[i] : 0u) << (8 * i);
-    const uint32_t a = e4m3x2_to_f16x2(w & 0xffffu), b = e4m3x2_to_f16x2(w >> 16);
-    const float f[4] = {f16lo_to_f32(a), f16hi_to_f32(a), f16lo_to_f32(b), f16hi_to_f32(b)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(__float2bfloat16_rn(__fmul_rn(f[i], inv)));
-  } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + row_off + k;
-    uint16_t h[4];
-    if (VEC) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      h[0] = w.x & 0xffffu; h[1] = w.x >> 16; h[2] = w.y & 0xffffu; h[3] = w.y >> 16;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = k + i < n ? p[i] : (uint16_t)0;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = T == QX_T_BF16 ? __uint_as_float((uint32_t)h[i] << 16) : __half2float(__ushort_as_half(h[i]));
   }
 }
 
-// round_half_even(p / m) for p = 127 x, 0 < m: the rounded estimate p * (1 / m)
-// is at most one off, and p - n m is exact for 8- and 11-bit x (p and n m both
-// fit 24 bits), so one comparison with half of m settles it; BF16 values often
-// sit on the half itself (x = m / 2 gives 63.5), where an inexact quotient would
-// fall to either side.
-__device__ __forceinline__ int quotient(float p, float m, float rm) {
-  float n = rintf(p * rm);
-  const float d = fmaf(-n, m, p), a2 = 2.f * fabsf(d);
-  if (a2 > m || (a2 == m && ((int)n & 1))) n += d > 0.f ? 1.f : -1.f;
-  return (int)fminf(fmaxf(n, -QMAX), QMAX);
+// 16 bytes of a row's elements from index k on; one load where the row is aligned
+// and the piece full, else element by element, those past n reading as 0.
+template <int T, bool VEC>
+__device__ __forceinline__ uint4 load16(const void* x, int64_t off, int k, int n) {
+  constexpr int E = per16<T>(), B = 16 / E;
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(x) + (off + k) * B;
+  if (VEC && k + E <= n) return __ldcg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    uint32_t e = 0u;
+    if (k + j < n) {
+      if constexpr (B == 4) e = reinterpret_cast<const uint32_t*>(p)[j];
+      else if constexpr (B == 2) e = reinterpret_cast<const uint16_t*>(p)[j];
+      else e = p[j];
+    }
+    w[j * B / 4] |= e << (8 * (j * B % 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int QTHR = 256;
+// round_half_even(p / m) for p = 127 x, 0 < m, as the low byte of the result: the
+// estimate p * (1 / m), rounded to a whole number by adding 1.5 * 2^23, is at most
+// one off, and p - n m is exact for 8- and 11-bit x (p and n m both fit 24 bits),
+// so one comparison with half of m settles it; BF16 values often sit on the half
+// itself (x = m / 2 gives 63.5), where an inexact quotient would fall to either side.
+__device__ __forceinline__ uint32_t quotient(float p, float m, float rm) {
+  constexpr float MAGIC = 12582912.f;
+  const float y = fmaf(p, rm, MAGIC), d = fmaf(MAGIC - y, m, p), a2 = 2.f * fabsf(d);
+  uint32_t n = __float_as_uint(y);
+  if (a2 >= m && (a2 > m || (n & 1u))) n += d > 0.f ? 1u : ~0u;
+  return n;
+}
+
+// Largest |x| of one 16-byte piece, as the bits of its type (16-bit types: of one of
+// two halves): a NaN or an infinity is above every number.
+template <int T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t m, const uint4& raw, float inv) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (T == QX_T_BF16 || T == QX_T_F16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  } else if constexpr (T == QX_T_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, w[i] & 0x7fffffffu);
+  } else {
+    float v[16];
+    unpack<T>(raw, inv, v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  return m;
+}
+
+// One CTA per row, about four 16-byte pieces per thread. The row is read once and
+// kept in registers (raw) between the maximum and the quantisation; what is longer
+// than NV pieces per thread is read again. Bound by the bytes. early: 1 lets the
+// kernels behind this one start before it has waited for the ones in front (their
+// weights are then known to be complete).
+constexpr int QTHR = 512, NV = 4;
 
 template <int T, bool VEC>
 __global__ void __launch_bounds__(QTHR) quant_kernel(const void* x, int64_t xs, const float* x_scale, int per_row,
-                                                     int k, int8_t* q, int64_t qs, float* scale) {
-  const int64_t r = blockIdx.x;
-  const float inv = T == QX_T_E4M3 ? x_scale[per_row ? r : 0] : 1.f;
-  float v[4];
-  uint32_t m = 0;                                  // |x| as bits: a NaN or infinity is the largest
-  for (int i = threadIdx.x * 4; i < k; i += QTHR * 4) {
-    load4<T, VEC>(x, r * xs, i, k, inv, v);
+                                                     int k, int8_t* q, int64_t qs, float* scale, int q_vec,
+                                                     int early) {
+  constexpr int E = per16<T>();
+  if (early) pdl_launch_dependents();
+  pdl_wait();
+  if (!early) pdl_launch_dependents();
+  const int64_t r = blockIdx.x, off = r * xs;
+  const float inv = T == QX_T_E4M3 ? __ldcg(&x_scale[per_row ? r : 0]) : 1.f;
+  const int pieces = (k + E - 1) / E, thr = blockDim.x;
+  uint4 raw[NV];
+  uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int i = 0; i < NV; ++i) {
+    const int g = threadIdx.x + i * thr;
+    raw[i] = g < pieces ? load16<T, VEC>(x, off, g * E, k) : make_uint4(0u, 0u, 0u, 0u);
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) m = top_bits<T>(m, raw[i], inv);
+  for (int g = threadIdx.x + NV * thr; g < pieces; g += thr) m = top_bits<T>(m, load16<T, VEC>(x, off, g * E, k), inv);
+  if constexpr (T == QX_T_BF16) m = max(m << 16, m & 0xffff0000u);
+  if constexpr (T == QX_T_F16)                     // FP16's largest as FP32 bits (infinity and NaN stay so)
+    m = __float_as_uint(__half2float(__ushort_as_half((uint16_t)max(m & 0xffffu, m >> 16))));
   m = __reduce_max_sync(0xffffffffu, m);
   __shared__ uint32_t sm[QTHR / 32];
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < QTHR / 32; ++i) m = max(m, sm[i]);
+  for (int i = 0; i < thr / 32; ++i) m = max(m, sm[i]);
   const bool bad = m >= INF_BITS;
   const float mc = fmaxf(__uint_as_float(m), AMAX_FLOOR);
   const float f = mc > 1e30f ? 0x1p-20f : 1.f;     // 127 x must not overflow: a power of two changes no quotient
   const float qm = QMAX * f, mf = mc * f, rm = __frcp_rn(mf);
+  const uint32_t keep = bad ? 0u : 0xffffffffu;
   if (threadIdx.x == 0) {
     scale[r] = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(mc, QMAX);
     if (bad) atomicOr(&g_status, (uint32_t)QX_DEV_NONFINITE);
   }
   int8_t* qr = q + r * qs;
-  for (int i = threadIdx.x * 4; i < k; i += QTHR * 4) {
-    load4<T, VEC>(x, r * xs, i, k, inv, v);
-    uint32_t w = 0;
+  auto put = [&](const uint4& w, int g) {
+    float v[E];
+    unpack<T>(w, inv, v);
+    uint32_t o[E / 4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w |= ((uint32_t)(bad ? 0 : quotient(__fmul_rn(v[j], qm), mf, rm)) & 0xffu) << (8 * j);
-    if (VEC) *reinterpret_cast<uint32_t*>(qr + i) = w;
-    else
+    for (int j = 0; j < E; j += 4) {
+      uint32_t n[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j < k) qr[i + j] = (int8_t)(w >> (8 * j));
-  }
+      for (int i = 0; i < 4; ++i) n[i] = quotient(__fmul_rn(v[j + i], qm), mf, rm);
+      o[j / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) & keep;
+    }
+    if (q_vec && (g + 1) * E <= k) {
+      if constexpr (E == 16) *reinterpret_cast<uint4*>(qr + g * E) = make_uint4(o[0], o[1], o[2], o[3]);
+      else if constexpr (E == 8) *reinterpret_cast<uint2*>(qr + g * E) = make_uint2(o[0], o[1]);
+      else *reinterpret_cast<uint32_t*>(qr + g * E) = o[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (g * E + j < k) qr[g * E + j] = (int8_t)(o[j / 4] >> (8 * (j % 4)));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (threadIdx.x + i * thr < pieces) put(raw[i], threadIdx.x + i * thr);
+  for (int g = threadIdx.x + NV * thr; g < pieces; g += thr) put(load16<T, VEC>(x, off, g * E, k), g);
 }
 
 // ------------------------------------------------------------------ product
@@ -164,6 +224,8 @@ struct Args {
 constexpr int ST = 64, SKB = 64;
 __global__ void __launch_bounds__(256) plain_kernel(Args p) {
   __shared__ __align__(16) int8_t sa[ST][SKB + 4], sw[ST][SKB + 4];
+  pdl_launch_dependents();
+  pdl_wait();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int half = p.swiglu ? ST / 2 : ST;               // output columns of the tile
   const int n0 = blockIdx.x * half, m0 = blockIdx.y * ST;
@@ -268,33 +330,49 @@ bool row_map(CUtensorMap* map, const int8_t* base, int64_t rows, int k, int64_t 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN>
-int split_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int pieces, cudaStream_t st) {
-  const int half = p.swiglu ? 64 : 128;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = pieces;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+// Every kernel here is launched so that it may start while the one in front of it
+// on the stream still runs (programmatic dependent launch): it sets itself up,
+// then waits for that one before it touches global memory.
+struct Launch {
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.n + half - 1) / half * pieces), (unsigned)((p.m + BN - 1) / BN), 1);
-  cfg.blockDim = dim3(SPLIT_THR, 1, 1);
-  cfg.dynamicSmemBytes = Split<BN>::SMEM;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, split_kernel<BN>, tw, ta, p, pieces, wait_limit_ns()) == cudaSuccess
-             ? QX_OK : QX_ERR_LAUNCH;
+  Launch(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster = 1) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+  }
+  template <typename... P, typename... A>
+  int operator()(void (*kernel)(P...), A... args) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
+  }
+};
+
+template <int BN>
+int split_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int pieces, int prefetch,
+                 cudaStream_t st) {
+  const int half = p.swiglu ? 64 : 128;
+  const dim3 grid((unsigned)((p.n + half - 1) / half * pieces), (unsigned)((p.m + BN - 1) / BN), 1);
+  return Launch(grid, SPLIT_THR, Split<BN>::SMEM, st, pieces)(split_kernel<BN>, tw, ta, p, pieces, prefetch,
+                                                            wait_limit_ns());
 }
 
 template <int BN>
-int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int sms, cudaStream_t st) {
+int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int prefetch, int sms, cudaStream_t st) {
   const int cols = p.swiglu ? BN / 2 : BN;
   const int tiles_m = (p.m + 255) / 256;
   const int64_t tiles = (int64_t)tiles_m * ((p.n + cols - 1) / cols);
   if (tiles > 0x7fffffff) return QX_ERR_SHAPE;
   const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
-  pair_kernel<BN><<<2 * pairs, PAIR_THR, Pair<BN>::SMEM, st>>>(tw, ta, p, tiles_m, (int)tiles, wait_limit_ns());
-  return cudaGetLastError() == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
+  return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, Pair<BN>::SMEM, st, 2)(pair_kernel<BN>, tw, ta, p, tiles_m,
+                                                                       (int)tiles, prefetch, wait_limit_ns());
 }
 
 // K pieces of the split kernel: the count (1..8) that leaves the busiest SM the
@@ -309,7 +387,7 @@ int pieces_of(int tiles, int chunks, int sms) {
   return best;
 }
 
-int tc_launch(const Args& p, int sms, cudaStream_t st) {
+int tc_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
   CUtensorMap tw, ta;
   const int64_t w_rows = p.swiglu ? 2ll * p.n : p.n;
   if (p.m <= 128) {
@@ -317,8 +395,10 @@ int tc_launch(const Args& p, int sms, cudaStream_t st) {
     if (!row_map(&tw, p.w, w_rows, p.k, p.ws, 64) || !row_map(&ta, p.a, p.m, p.k, p.as, bn)) return QX_ERR_DEVICE;
     const int half = p.swiglu ? 64 : 128;
     const int s = pieces_of((p.n + half - 1) / half, (p.k + (int)KST - 1) / (int)KST, sms);
-    return bn == 16 ? split_launch<16>(p, tw, ta, s, st) : bn == 32 ? split_launch<32>(p, tw, ta, s, st)
-         : bn == 64 ? split_launch<64>(p, tw, ta, s, st) : split_launch<128>(p, tw, ta, s, st);
+    return bn == 16   ? split_launch<16>(p, tw, ta, s, prefetch, st)
+           : bn == 32 ? split_launch<32>(p, tw, ta, s, prefetch, st)
+           : bn == 64 ? split_launch<64>(p, tw, ta, s, prefetch, st)
+                      : split_launch<128>(p, tw, ta, s, prefetch, st);
   }
   // 256 or 128 weight rows per tile: whichever leaves the busiest pair fewer of them
   const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, h = p.swiglu ? 2 : 1;
@@ -328,53 +408,104 @@ int tc_launch(const Args& p, int sms, cudaStream_t st) {
   };
   const int bn = waves(128) < waves(256) ? 128 : 256;
   if (!row_map(&tw, p.w, w_rows, p.k, p.ws, bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, 128)) return QX_ERR_DEVICE;
-  return bn == 128 ? pair_launch<128>(p, tw, ta, sms, st) : pair_launch<256>(p, tw, ta, sms, st);
+  return bn == 128 ? pair_launch<128>(p, tw, ta, prefetch, sms, st) : pair_launch<256>(p, tw, ta, prefetch, sms, st);
+}
+
+// A checked product. prefetch: the weights are complete when this kernel starts,
+// so their copies may go out before it waits for the kernel in front.
+int product(Args p, int prefetch, int sms, cudaStream_t st) {
+  // Tiled copies need rows that start on 16-byte boundaries (a single row: its address only).
+  auto aligned = [](const int8_t* b, int64_t stride, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(b) % 16 == 0 && (stride % 16 == 0 || rows == 1);
+  };
+  if (aligned(p.a, p.as, p.m) && aligned(p.w, p.ws, p.swiglu ? 2 : p.n)) {
+    if (p.m == 1) p.as = (p.as + 15) / 16 * 16;          // never stepped
+    if (p.n == 1 && !p.swiglu) p.ws = (p.ws + 15) / 16 * 16;
+    return tc_launch(p, prefetch, sms, st);
+  }
+  const int half = p.swiglu ? ST / 2 : ST;
+  const int64_t gy = (p.m + ST - 1) / ST;
+  if (gy > 65535) return QX_ERR_SHAPE;
+  return Launch(dim3((unsigned)((p.n + half - 1) / half), (unsigned)gy, 1), 256, 0, st)(plain_kernel, p);
 }
 
 template <int T>
-void quant_launch(const void* x, int64_t xs, const float* x_scale, int per_row, int64_t rows, int k, int8_t* q,
-                  int64_t qs, float* scale, bool vec, cudaStream_t st) {
-  if (vec) quant_kernel<T, true><<<(unsigned)rows, QTHR, 0, st>>>(x, xs, x_scale, per_row, k, q, qs, scale);
-  else quant_kernel<T, false><<<(unsigned)rows, QTHR, 0, st>>>(x, xs, x_scale, per_row, k, q, qs, scale);
+int quant_launch(const void* x, int64_t xs, const float* x_scale, int per_row, int64_t rows, int k, int8_t* q,
+                 int64_t qs, float* scale, int early, cudaStream_t st) {
+  constexpr int E = per16<T>(), B = 16 / E;
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && xs * B % 16 == 0;
+  const int q_vec = reinterpret_cast<uintptr_t>(q) % E == 0 && qs % E == 0;
+  const int pieces = (k + E - 1) / E, want = ((pieces + NV - 1) / NV + 31) / 32 * 32;
+  Launch l(dim3((unsigned)rows, 1, 1), want < QTHR ? want : QTHR, 0, st);
+  return vec ? l(quant_kernel<T, true>, x, xs, x_scale, per_row, k, q, qs, scale, q_vec, early)
+             : l(quant_kernel<T, false>, x, xs, x_scale, per_row, k, q, qs, scale, q_vec, early);
 }
+
+int quantise(const void* x, int64_t xs, int type, const float* x_scale, int per_row, int64_t rows, int k, int8_t* q,
+             int64_t qs, float* scale, int early, cudaStream_t st) {
+  if (type == QX_T_BF16) return quant_launch<QX_T_BF16>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
+  if (type == QX_T_F16) return quant_launch<QX_T_F16>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
+  if (type == QX_T_F32) return quant_launch<QX_T_F32>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
+  return quant_launch<QX_T_E4M3>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
+}
+
+int element_size(int type) { return type == QX_T_F32 ? 4 : type == QX_T_E4M3 ? 1 : 2; }
+
+int check_x(const void* x, int64_t x_stride, int type, const float* x_scale, int64_t n_scale, int64_t rows, int k) {
+  if (!x) return QX_ERR_ARG;
+  if (type == QX_T_E4M3 && (!x_scale || (n_scale != 1 && n_scale != rows))) return QX_ERR_ARG;
+  if (x_stride < k) return QX_ERR_SHAPE;
+  return reinterpret_cast<uintptr_t>(x) % element_size(type) ? QX_ERR_ALIGN : QX_OK;
+}
+
+constexpr int MAX_DIM = 1 << 24;
+
+// Rows of q, its scales, h, q2 and its scales in an expert's workspace, each on a
+// 16-byte boundary with rows a multiple of 16 bytes apart.
+struct ExpertLayout {
+  int64_t qs, hs, q2s;
+  size_t q, s, h, q2, s2, total;
+  ExpertLayout(int64_t rows, int k, int inter) {
+    qs = (k + 15) / 16 * 16;
+    hs = (inter + 3) / 4 * 4;
+    q2s = (inter + 15) / 16 * 16;
+    auto al = [](size_t v) { return (v + 255) & ~size_t(255); };
+    q = 0;
+    s = al(q + (size_t)rows * qs);
+    h = al(s + (size_t)rows * 4);
+    q2 = al(h + (size_t)rows * hs * 4);
+    s2 = al(q2 + (size_t)rows * q2s);
+    total = al(s2 + (size_t)rows * 4);
+  }
+};
 }  // namespace
 
 extern "C" {
 
-int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* x_scale, int32_t n_scale,
+int qx_quant_int8(const void* x, int64_t x_stride, int32_t x_type, const float* x_scale, int64_t n_scale,
                   int64_t rows, int32_t k, int8_t* q, int64_t q_stride, float* scale, void* stream) {
   if (rows < 0 || rows > 0x7fffffffll || k < 1 || k > QX_INT8_MAX_K) return QX_ERR_SHAPE;
   if (x_type < QX_T_BF16 || x_type > QX_T_E4M3) return QX_ERR_ARG;
   if (rows == 0) return QX_OK;
-  if (!x || !q || !scale) return QX_ERR_ARG;
-  if (x_type == QX_T_E4M3 && (!x_scale || (n_scale != 1 && n_scale != rows))) return QX_ERR_ARG;
-  if (x_stride < k || q_stride < k) return QX_ERR_SHAPE;
-  const int esz = x_type == QX_T_F32 ? 4 : x_type == QX_T_E4M3 ? 1 : 2;
-  if (reinterpret_cast<uintptr_t>(x) % esz || reinterpret_cast<uintptr_t>(scale) % 4) return QX_ERR_ALIGN;
+  if (!q || !scale) return QX_ERR_ARG;
+  if (const int rc = check_x(x, x_stride, x_type, x_scale, n_scale, rows, k)) return rc;
+  if (q_stride < k) return QX_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(scale) % 4) return QX_ERR_ALIGN;
   if (device_sms() <= 0) return QX_ERR_DEVICE;
-  // four elements per access where every row starts on that boundary and has a multiple of four
-  const bool vec = k % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * esz) == 0 && x_stride % 4 == 0 &&
-                   reinterpret_cast<uintptr_t>(q) % 4 == 0 && q_stride % 4 == 0;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int per_row = n_scale == rows && rows > 1;
-  if (x_type == QX_T_BF16) quant_launch<QX_T_BF16>(x, x_stride, x_scale, per_row, rows, k, q, q_stride, scale, vec, st);
-  else if (x_type == QX_T_F16) quant_launch<QX_T_F16>(x, x_stride, x_scale, per_row, rows, k, q, q_stride, scale, vec, st);
-  else if (x_type == QX_T_F32) quant_launch<QX_T_F32>(x, x_stride, x_scale, per_row, rows, k, q, q_stride, scale, vec, st);
-  else quant_launch<QX_T_E4M3>(x, x_stride, x_scale, per_row, rows, k, q, q_stride, scale, vec, st);
-  return cudaGetLastError() == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
+  return quantise(x, x_stride, x_type, x_scale, n_scale == rows, rows, k, q, q_stride, scale, 0,
+                  reinterpret_cast<cudaStream_t>(stream));
 }
 
 int qx_int8_matmul(const QxInt8Args* a, void* stream) {
   if (!a) return QX_ERR_ARG;
-  if (a->m < 0 || a->n < 1 || a->n > (1 << 24) || a->m > (1 << 24) || a->k < 1 || a->k > QX_INT8_MAX_K)
+  if (a->m < 0 || a->n < 1 || a->n > MAX_DIM || a->m > MAX_DIM || a->k < 1 || a->k > QX_INT8_MAX_K)
     return QX_ERR_SHAPE;
   if (a->out_type < QX_T_BF16 || a->out_type > QX_T_F32) return QX_ERR_ARG;
   if (a->m == 0) return QX_OK;
   if (!a->a || !a->w || !a->a_scale || !a->w_scale || !a->out) return QX_ERR_ARG;
   if (a->a_stride < a->k || a->w_stride < a->k || a->out_stride < a->n) return QX_ERR_SHAPE;
-  const int osz = a->out_type == QX_T_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(a->out) % osz || reinterpret_cast<uintptr_t>(a->a_scale) % 4 ||
-      reinterpret_cast<uintptr_t>(a->w_scale) % 4)
+  if (reinterpret_cast<uintptr_t>(a->out) % element_size(a->out_type) ||
+      reinterpret_cast<uintptr_t>(a->a_scale) % 4 || reinterpret_cast<uintptr_t>(a->w_scale) % 4)
     return QX_ERR_ALIGN;
   const int sms = device_sms();
   if (sms <= 0) return QX_ERR_DEVICE;
@@ -383,21 +514,56 @@ int qx_int8_matmul(const QxInt8Args* a, void* stream) {
   p.as = a->a_stride; p.ws = a->w_stride; p.os = a->out_stride;
   p.m = a->m; p.n = a->n; p.k = a->k; p.type = a->out_type;
   p.swiglu = a->swiglu ? 1 : 0; p.has_limit = a->has_limit ? 1 : 0; p.limit = a->limit;
+  return product(p, 0, sms, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t qx_int8_expert_workspace_bytes(int32_t rows, int32_t k, int32_t inter) {
+  if (rows < 0 || rows > MAX_DIM || k < 1 || k > QX_INT8_MAX_K || inter < 1 || inter > QX_INT8_MAX_K) return 0;
+  return ExpertLayout(rows, k, inter).total;
+}
+
+int qx_int8_expert(const QxInt8ExpertArgs* a, void* stream) {
+  if (!a) return QX_ERR_ARG;
+  if (a->rows < 0 || a->rows > MAX_DIM || a->k < 1 || a->k > QX_INT8_MAX_K || a->inter < 1 ||
+      a->inter > QX_INT8_MAX_K)
+    return QX_ERR_SHAPE;
+  if (a->x_type < QX_T_BF16 || a->x_type > QX_T_E4M3 || a->out_type < QX_T_BF16 || a->out_type > QX_T_F32)
+    return QX_ERR_ARG;
+  if (a->rows == 0) return QX_OK;
+  if (!a->w13 || !a->w13_scale || !a->w2 || !a->w2_scale || !a->out || !a->workspace) return QX_ERR_ARG;
+  if (const int rc = check_x(a->x, a->x_stride, a->x_type, a->x_scale, a->n_scale, a->rows, a->k)) return rc;
+  if (a->w13_stride < a->k || a->w2_stride < a->inter || a->out_stride < a->k) return QX_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(a->out) % element_size(a->out_type) ||
+      reinterpret_cast<uintptr_t>(a->w13_scale) % 4 || reinterpret_cast<uintptr_t>(a->w2_scale) % 4 ||
+      reinterpret_cast<uintptr_t>(a->workspace) % 16)
+    return QX_ERR_ALIGN;
+  const ExpertLayout L(a->rows, a->k, a->inter);
+  if (a->workspace_bytes < L.total) return QX_ERR_WORKSPACE;
+  const int sms = device_sms();
+  if (sms <= 0) return QX_ERR_DEVICE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // Tiled copies need rows that start on 16-byte boundaries (a single row: its address only).
-  auto aligned = [](const int8_t* b, int64_t stride, int64_t rows) {
-    return reinterpret_cast<uintptr_t>(b) % 16 == 0 && (stride % 16 == 0 || rows == 1);
-  };
-  if (aligned(p.a, p.as, p.m) && aligned(p.w, p.ws, p.swiglu ? 2 : p.n)) {
-    if (p.m == 1) p.as = (p.as + 15) / 16 * 16;          // never stepped
-    if (p.n == 1 && !p.swiglu) p.ws = (p.ws + 15) / 16 * 16;
-    return tc_launch(p, sms, st);
-  }
-  const int half = p.swiglu ? ST / 2 : ST;
-  const int64_t gy = (p.m + ST - 1) / ST;
-  if (gy > 65535) return QX_ERR_SHAPE;
-  plain_kernel<<<dim3((unsigned)((p.n + half - 1) / half), (unsigned)gy), 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? QX_OK : QX_ERR_LAUNCH;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
+  Args p;
+  p.a = reinterpret_cast<int8_t*>(ws + L.q); p.as = L.qs; p.sa = reinterpret_cast<float*>(ws + L.s);
+  p.w = a->w13; p.ws = a->w13_stride; p.sw = a->w13_scale;
+  p.out = ws + L.h; p.os = L.hs; p.type = QX_T_F32;
+  p.m = a->rows; p.n = a->inter; p.k = a->k;
+  p.swiglu = 1; p.has_limit = a->has_limit ? 1 : 0; p.limit = a->limit;
+  Args d = p;
+  d.a = reinterpret_cast<int8_t*>(ws + L.q2); d.as = L.q2s; d.sa = reinterpret_cast<float*>(ws + L.s2);
+  d.w = a->w2; d.ws = a->w2_stride; d.sw = a->w2_scale;
+  d.out = a->out; d.os = a->out_stride; d.type = a->out_type;
+  d.n = a->k; d.k = a->inter; d.swiglu = 0;
+  int rc = quantise(a->x, a->x_stride, a->x_type, a->x_scale, a->n_scale == a->rows, a->rows, a->k,
+                    reinterpret_cast<int8_t*>(ws + L.q), L.qs, reinterpret_cast<float*>(ws + L.s), 0, st);
+  // The first quantiser lets the products start only after everything queued before
+  // this call is complete, the weights included: their copies go out at once.
+  if (rc == QX_OK) rc = product(p, 1, sms, st);
+  if (rc == QX_OK)
+    rc = quantise(ws + L.h, L.hs, QX_T_F32, nullptr, 0, a->rows, a->inter, reinterpret_cast<int8_t*>(ws + L.q2), L.q2s,
+                  reinterpret_cast<float*>(ws + L.s2), 1, st);
+  if (rc == QX_OK) rc = product(d, 1, sms, st);
+  return rc;
 }
 
 int qx_int8_status(uint32_t* status, void* stream) {

@@ -147,6 +147,32 @@ class QxInt8Args(ctypes.Structure):
     ]
 
 
+class QxInt8ExpertArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_type", ctypes.c_int32),
+        ("n_scale", ctypes.c_int32),
+        ("x_scale", ctypes.c_void_p),
+        ("w13", ctypes.c_void_p),
+        ("w13_stride", ctypes.c_int64),
+        ("w13_scale", ctypes.c_void_p),
+        ("w2", ctypes.c_void_p),
+        ("w2_stride", ctypes.c_int64),
+        ("w2_scale", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("out_type", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("inter", ctypes.c_int32),
+        ("has_limit", ctypes.c_int32),
+        ("limit", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point in include/qmesh_b200.h
 SIGNATURES = [
     ("qx_arena_w13_bytes", ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
@@ -201,9 +227,11 @@ SIGNATURES = [
      [ctypes.POINTER(QxArena), ctypes.POINTER(QxSliceArgs), ctypes.POINTER(QxRouterArgs), ctypes.POINTER(QxArena),
       ctypes.c_void_p]),
     ("qx_quant_int8", ctypes.c_int,
-     [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
+     [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
       ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
     ("qx_int8_matmul", ctypes.c_int, [ctypes.POINTER(QxInt8Args), ctypes.c_void_p]),
+    ("qx_int8_expert_workspace_bytes", ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    ("qx_int8_expert", ctypes.c_int, [ctypes.POINTER(QxInt8ExpertArgs), ctypes.c_void_p]),
     ("qx_int8_status", ctypes.c_int, [ctypes.POINTER(ctypes.c_uint32), ctypes.c_void_p]),
     ("qx_combine_p2p", ctypes.c_int, [ctypes.POINTER(QxXchgArgs), ctypes.c_void_p]),
     ("qx_version", ctypes.c_char_p, []),

@@ -18,8 +18,7 @@ import torch
 from . import _lib
 from .arena import Arena
 from .expert_slice import SWIGLU_LIMIT, _slice_args
-from .int8 import Int8Expert, _on, _p, _same_device
-from .trace import rng
+from .int8 import Int8Expert, launch_on, same_device
 
 
 def workspace_bytes(rows: int, n_experts: int, topk: int, c0: int, c1: int) -> int:
@@ -65,9 +64,9 @@ def moe_layer(arena: Arena, li: int, x: torch.Tensor, gate: torch.Tensor, bias: 
     c0 = arena.a0 if c0 is None else c0
     c1 = arena.a1 if c1 is None else c1
     view = arena.view(li)
-    if dev.type != "cuda" or dev != arena.w13[li].device:
+    if dev != arena.w13[li].device:
         raise ValueError(f"x is on {dev}, the arena on {arena.w13[li].device}")
-    _same_device(dev, gate=gate, bias=bias, ids=ids, tw=tw, x_scale=x_scale, out=out, workspace=workspace)
+    same_device(dev, gate=gate, bias=bias, ids=ids, tw=tw, x_scale=x_scale, out=out, workspace=workspace)
     if out is None:
         out = torch.empty(rows, _lib.HIDDEN, dtype=torch.bfloat16, device=dev)
     if workspace is None:
@@ -80,12 +79,10 @@ def moe_layer(arena: Arena, li: int, x: torch.Tensor, gate: torch.Tensor, bias: 
         shared = None
     args = _slice_args(x, None, None, out, c0, c1, workspace, x_scale, max(swiglu_limit, 0.0), swiglu_limit > 0,
                        topk=topk)
-    router = _lib.QxRouterArgs(_p(gate), _lib.QX_T_BF16 if gate.dtype == torch.bfloat16 else _lib.QX_T_F32,
-                               gate.stride(0), _p(bias), _p(ids), _p(tw), _p(addend),
-                               addend.stride(0) if addend is not None else 0)
-    with _on(dev), rng("qx.moe_layer"):
-        rc = _lib.load().qx_moe_decode_tc(ctypes.byref(view), ctypes.byref(args), ctypes.byref(router),
-                                          ctypes.byref(shared) if shared is not None else None,
-                                          ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-    _lib.check(rc, "qx_moe_decode_tc")
+    router = _lib.QxRouterArgs(
+        gate.data_ptr(), _lib.QX_T_BF16 if gate.dtype == torch.bfloat16 else _lib.QX_T_F32, gate.stride(0),
+        bias.data_ptr() if bias is not None else 0, ids.data_ptr() if ids is not None else 0,
+        tw.data_ptr() if tw is not None else 0, addend.data_ptr() if addend is not None else 0, _lib.HIDDEN)
+    launch_on(dev, _lib.load().qx_moe_decode_tc, "qx_moe_decode_tc", ctypes.byref(view), ctypes.byref(args),
+              ctypes.byref(router), ctypes.byref(shared) if shared is not None else None)
     return out

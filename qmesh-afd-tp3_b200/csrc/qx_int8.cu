@@ -299,8 +299,8 @@ int device_sms() {
       cudaFuncSetAttribute(split_kernel<32>, attr, (int)Split<32>::SMEM) != cudaSuccess ||
       cudaFuncSetAttribute(split_kernel<64>, attr, (int)Split<64>::SMEM) != cudaSuccess ||
       cudaFuncSetAttribute(split_kernel<128>, attr, (int)Split<128>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(pair_kernel<128>, attr, (int)Pair<128>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(pair_kernel<256>, attr, (int)Pair<256>::SMEM) != cudaSuccess)
+      cudaFuncSetAttribute(pair_kernel<1>, attr, (int)Pair<1>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(pair_kernel<2>, attr, (int)Pair<2>::SMEM) != cudaSuccess)
     return 0;
   return cached[dev] = sms;
 }
@@ -311,9 +311,12 @@ uint64_t wait_limit_ns() {
   return (uint64_t)(ms < 10 ? 10 : ms) * 1000000ull;
 }
 
-// Tiled-copy descriptor of int8 rows [rows, k], boxes of 128 bytes x box_rows with
-// the 128-byte swizzle; places outside the tensor read as 0.
-bool row_map(CUtensorMap* map, const int8_t* base, int64_t rows, int k, int64_t stride, int box_rows) {
+int element_size(int type) { return type == QX_T_F32 ? 4 : type == QX_T_E4M3 ? 1 : 2; }
+
+// Tiled-copy descriptor of rows x cols elements of 1, 2 or 4 bytes; places outside
+// the tensor read as 0 and are not written.
+bool tiled_map(CUtensorMap* map, const void* base, int esz, int64_t rows, int64_t cols, int64_t stride_bytes, int box_cols,
+               int box_rows, CUtensorMapSwizzle swizzle) {
   static decltype(&cuTensorMapEncodeTiled) encode = [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult res;
@@ -323,11 +326,18 @@ bool row_map(CUtensorMap* map, const int8_t* base, int64_t rows, int k, int64_t 
     return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
   }();
   if (!encode) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t box[2] = {KST, (cuuint32_t)box_rows}, one[2] = {1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, one,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const CUtensorMapDataType type = esz == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : esz == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Of int8 rows [rows, k]: boxes of one 128-byte swizzle span x box_rows.
+bool row_map(CUtensorMap* map, const int8_t* base, int64_t rows, int k, int64_t stride, int box_rows) {
+  return tiled_map(map, base, 1, rows, k, stride, KST, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Every kernel here is launched so that it may start while the one in front of it
@@ -364,15 +374,46 @@ int split_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, in
                                                             wait_limit_ns());
 }
 
-template <int BN>
-int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int prefetch, int sms, cudaStream_t st) {
-  const int cols = p.swiglu ? BN / 2 : BN;
-  const int tiles_m = (p.m + 255) / 256;
-  const int64_t tiles = (int64_t)tiles_m * ((p.n + cols - 1) / cols);
-  if (tiles > 0x7fffffff) return QX_ERR_SHAPE;
-  const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
-  return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, Pair<BN>::SMEM, st, 2)(pair_kernel<BN>, tw, ta, p, tiles_m,
-                                                                       (int)tiles, prefetch, wait_limit_ns());
+// Tile of the pair kernel: 256 mt tokens x bn weight rows.
+struct PairTile {
+  int mt, bn, tiles_m;
+  int64_t tiles;
+};
+
+// The tile with the smallest estimated time: waves of tiles over the pairs, each
+// 128-byte chunk of K taking the longer of its MMAs (335 ns for 256 x 256, measured
+// without copies) and its copies (both CTAs' operands of every busy pair at 11.5
+// TB/s, measured), and an epilogue (1.4 us for 256 x 256) that only one block per
+// tile hides, but for the last.
+PairTile pair_tile(const Args& p, int sms) {
+  const int pairs = sms / 2, chunks = (p.k + (int)KST - 1) / (int)KST, h = p.swiglu ? 2 : 1, step = 32 * h;
+  PairTile best = {};
+  double least = 0;
+  for (int mt = 1; mt <= 2; ++mt) {
+    for (int bn = 2 * step; bn <= 256; bn += step) {
+      PairTile t = {mt, bn, (p.m + 256 * mt - 1) / (256 * mt), 0};
+      t.tiles = (int64_t)t.tiles_m * ((p.n + bn / h - 1) / (bn / h));
+      const double waves = (double)((t.tiles + pairs - 1) / pairs), busy = (double)(t.tiles < pairs ? t.tiles : pairs);
+      const double mma = 335.0 * mt * bn / 256, copy = (mt * 16384 + bn * 64) * 2 * busy / 11500.0;
+      const double epi = 1400.0 * bn / 256, loop = chunks * (mma > copy ? mma : copy);
+      const double ns = mt == 1 ? waves * (loop > epi ? loop : epi) + epi : waves * (loop + epi);
+      if (best.mt == 0 || ns < least) best = t, least = ns;
+    }
+  }
+  return best;
+}
+
+template <int MT>
+int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, const PairTile& t, int prefetch, int sms,
+                cudaStream_t st) {
+  if (t.tiles > 0x7fffffff) return QX_ERR_SHAPE;
+  const int pairs = (int)(t.tiles < sms / 2 ? t.tiles : sms / 2), osz = element_size(p.type);
+  // Tiled stores where the output's rows start on 16-byte boundaries.
+  CUtensorMap to = {};
+  const int tma = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.os * osz % 16 == 0 &&
+                  tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+  return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, Pair<MT>::SMEM, st, 2)(pair_kernel<MT>, tw, ta, to, p, t.bn, t.tiles_m,
+                                                                       (int)t.tiles, prefetch, tma, wait_limit_ns());
 }
 
 // K pieces of the split kernel: the count (1..8) that leaves the busiest SM the
@@ -400,15 +441,9 @@ int tc_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
            : bn == 64 ? split_launch<64>(p, tw, ta, s, prefetch, st)
                       : split_launch<128>(p, tw, ta, s, prefetch, st);
   }
-  // 256 or 128 weight rows per tile: whichever leaves the busiest pair fewer of them
-  const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, h = p.swiglu ? 2 : 1;
-  auto waves = [&](int bn) {
-    const int64_t t = (int64_t)tiles_m * ((p.n * (int64_t)h + bn - 1) / bn);
-    return (t + pairs - 1) / pairs * bn;
-  };
-  const int bn = waves(128) < waves(256) ? 128 : 256;
-  if (!row_map(&tw, p.w, w_rows, p.k, p.ws, bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, 128)) return QX_ERR_DEVICE;
-  return bn == 128 ? pair_launch<128>(p, tw, ta, prefetch, sms, st) : pair_launch<256>(p, tw, ta, prefetch, sms, st);
+  const PairTile t = pair_tile(p, sms);
+  if (!row_map(&tw, p.w, w_rows, p.k, p.ws, t.bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, 128)) return QX_ERR_DEVICE;
+  return t.mt == 1 ? pair_launch<1>(p, tw, ta, t, prefetch, sms, st) : pair_launch<2>(p, tw, ta, t, prefetch, sms, st);
 }
 
 // A checked product. prefetch: the weights are complete when this kernel starts,
@@ -448,8 +483,6 @@ int quantise(const void* x, int64_t xs, int type, const float* x_scale, int per_
   if (type == QX_T_F32) return quant_launch<QX_T_F32>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
   return quant_launch<QX_T_E4M3>(x, xs, x_scale, per_row, rows, k, q, qs, scale, early, st);
 }
-
-int element_size(int type) { return type == QX_T_F32 ? 4 : type == QX_T_E4M3 ? 1 : 2; }
 
 int check_x(const void* x, int64_t x_stride, int type, const float* x_scale, int64_t n_scale, int64_t rows, int k) {
   if (!x) return QX_ERR_ARG;

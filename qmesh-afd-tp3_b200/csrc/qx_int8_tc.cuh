@@ -81,12 +81,14 @@ __device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
   return v;
 }
+// Arrive on another CTA's barrier. CTA scope: it says that accumulator reads are
+// done and publishes no memory; at cluster scope it would first wait for this
+// thread's global stores (1,400 cycles per tile).
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Arrive on `bar` in both CTAs of the pair when the tcgen05 operations issued so far are done.
 __device__ __forceinline__ void commit_pair(uint64_t* bar) {
@@ -97,13 +99,13 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       : "memory");
 }
 
-// Bounded wait (cluster scope): false once the deadline has passed, with
+// Bounded wait: false once the deadline has passed, with
 // QX_DEV_TIMEOUT recorded; the caller then stops consuming.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint64_t deadline) {
   for (uint32_t it = 0;; ++it) {
     uint32_t ok;
     asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
@@ -263,14 +265,22 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   const bool vec = reinterpret_cast<uintptr_t>(p.out) % four == 0 && p.os % 4 == 0;
   for (int i = i0 + (int)threadIdx.x; i < i1; i += SPLIT_THR) {
     const int t = i / per, r = (i - t * per) * 4, n = n0 + r;
-    int4 g = make_int4(0, 0, 0, 0), u = g;
-    for (int s = 0; s < pieces; ++s) {
-      const uint32_t at = (pieces > 1 ? mapa(mine, s) : mine) + (uint32_t)(t * 128 + r) * 4u;
-      const int4 a = ld_cluster_int4(at);
-      g.x += a.x; g.y += a.y; g.z += a.z; g.w += a.w;
-      if (p.swiglu) {
-        const int4 b = ld_cluster_int4(at + 64 * 4);
-        u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
+    const uint32_t own = mine + (uint32_t)(t * 128 + r) * 4u;
+    int4 part[8], up[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {                          // every piece's sums requested at once
+      if (s < pieces) {
+        const uint32_t from = pieces > 1 ? mapa(own, s) : own;
+        part[s] = ld_cluster_int4(from);
+        if (p.swiglu) up[s] = ld_cluster_int4(from + 64 * 4);
+      }
+    }
+    int4 g = part[0], u = up[0];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) {
+      if (s < pieces) {
+        g.x += part[s].x; g.y += part[s].y; g.z += part[s].z; g.w += part[s].w;
+        if (p.swiglu) { u.x += up[s].x; u.y += up[s].y; u.z += up[s].z; u.w += up[s].w; }
       }
     }
     const float sa = __ldcg(&p.sa[m0 + t]);
@@ -309,53 +319,61 @@ __device__ __forceinline__ bool epilogue_and(bool pred) {
   return r != 0u;
 }
 
-// Staging row of one token: 32 outputs, padded so that 16-byte accesses of
-// consecutive rows fall into different banks (144 bytes for FP32, 80 for 16-bit types).
-constexpr int PAIR_ROW = 32 * 4 + 16;
+// Output staging of one epilogue warp: 32 tokens x 64 bytes (32 outputs of a 16-bit
+// type, 16 FP32), 16-byte pieces permuted as the copy engine's 64-byte swizzle does
+// (piece j of row r at j ^ (r / 2 mod 4)), which also keeps the lanes' accesses in
+// different banks. Two buffers, so that a store drains while the next block is written.
+constexpr int PAIR_BLOCK = 32 * 64;
 
-// 32 tokens x 32 output columns from column n on, each lane holding its token's
-// values: through shared memory, so that a warp's stores cover whole row segments
-// (16 bytes per lane where the rows are aligned, else one element per lane).
-__device__ __forceinline__ void store_block(const Args& p, uint8_t* stage, int64_t row0, int n, const float (&v)[32],
-                                            bool vec, int lane) {
-  const bool wide = p.type == QX_T_F32;
-  const int rowb = wide ? PAIR_ROW : 32 * 2 + 16;
-  uint8_t* mine = stage + lane * rowb;
-  if (wide) {
+// 32 tokens x COLS output columns from column n on, each lane holding its token's
+// values. Rows on 16-byte boundaries (tma): one tiled store, which leaves out what
+// lies past the tensor's end; else element by element, 64 bytes of a row at a time.
+template <int COLS>
+__device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to, uint8_t* stage, int64_t row0, int n,
+                                            const float* v, bool tma, int lane) {
+  constexpr int OSZ = 64 / COLS;
+  uint8_t* mine = stage + lane * 64;
+  const int sw = (lane >> 1) & 3;
+  if (tma) {                                             // the store before last has left this buffer
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+  }
 #pragma unroll
-    for (int j = 0; j < 32; j += 4)
-      *reinterpret_cast<float4*>(mine + 4 * j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8)
-      *reinterpret_cast<uint4*>(mine + 2 * j) =
-          make_uint4(pack2(p.type, v[j], v[j + 1]), pack2(p.type, v[j + 2], v[j + 3]), pack2(p.type, v[j + 4], v[j + 5]),
-                     pack2(p.type, v[j + 6], v[j + 7]));
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (OSZ == 4)
+      *reinterpret_cast<float4*>(mine + 16 * (j ^ sw)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    else
+      *reinterpret_cast<uint4*>(mine + 16 * (j ^ sw)) =
+          make_uint4(pack2(p.type, v[8 * j], v[8 * j + 1]), pack2(p.type, v[8 * j + 2], v[8 * j + 3]),
+                     pack2(p.type, v[8 * j + 4], v[8 * j + 5]), pack2(p.type, v[8 * j + 6], v[8 * j + 7]));
+  }
+  if (tma) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(to), "r"(n),
+                   "r"((int)row0), "r"(smem_u32(stage))
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    return;
   }
   __syncwarp();
-  const int rows = (int)min((int64_t)32, p.m - row0), cols = min(32, p.n - n);
-  const int osz = wide ? 4 : 2;
-  uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + (row0 * p.os + n) * osz;
-  if (vec && cols == 32) {
-    const int per = wide ? 8 : 4, part = lane % per;      // lanes per row segment
+  const int rows = (int)min((int64_t)32, p.m - row0), c = lane % COLS;
+  const int64_t step = p.os * OSZ;
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + row0 * step + (int64_t)(n + c) * OSZ;
+  if (n + c < p.n) {
 #pragma unroll 4
-    for (int r = lane / per; r < rows; r += 32 / per)
-      *reinterpret_cast<uint4*>(out + (int64_t)r * p.os * osz + part * 16) =
-          *reinterpret_cast<const uint4*>(stage + r * rowb + part * 16);
-  } else if (lane < cols) {
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      if (wide) *reinterpret_cast<float*>(out + ((int64_t)r * p.os + lane) * 4) =
-                    *reinterpret_cast<const float*>(stage + r * rowb + lane * 4);
-      else *reinterpret_cast<uint16_t*>(out + ((int64_t)r * p.os + lane) * 2) =
-               *reinterpret_cast<const uint16_t*>(stage + r * rowb + lane * 2);
+    for (int r = lane / COLS; r < rows; r += 32 / COLS) {
+      const uint8_t* from = stage + r * 64 + 16 * ((c * OSZ / 16) ^ ((r >> 1) & 3)) + c * OSZ % 16;
+      if constexpr (OSZ == 4) *reinterpret_cast<float*>(out + r * step) = *reinterpret_cast<const float*>(from);
+      else *reinterpret_cast<uint16_t*>(out + r * step) = *reinterpret_cast<const uint16_t*>(from);
     }
   }
   __syncwarp();
 }
 
-// Epilogue warps: two per quarter of the accumulator's lanes, each half of the columns
-// (one per quarter kept the tensor cores waiting: 87 us against 79 at 8192 x 5120 x 2304).
+// Epilogue warps: two per quarter of the accumulator's lanes.
 constexpr int PAIR_EPI = 8;
 
 // The scaled values of two neighbouring columns (packed multiplications, each
@@ -372,36 +390,41 @@ __device__ __forceinline__ float2 scaled2(int32_t a, int32_t b, float sa, float2
   return r;
 }
 
-template <int BN>
+// MT: 256-token blocks per tile. One block leaves room for two accumulators, so a
+// tile's epilogue runs under the next one's MMAs; two blocks share every weight
+// copy, which brings the copies below the MMAs' time, with no second accumulator.
+template <int MT>
 struct Pair {
-  static constexpr uint32_t A_BYTES = 128 * KST, B_BYTES = BN / 2 * KST, STAGE = A_BYTES + B_BYTES;
-  static constexpr int NS = BN == 256 ? 5 : 7;
-  static constexpr uint32_t COLS = 2 * BN;
-  // ring, the epilogue warps' staging rows, alignment of the swizzled tiles
-  static constexpr size_t SMEM = NS * STAGE + PAIR_EPI * 32 * PAIR_ROW + 1024;
+  static constexpr uint32_t A_BYTES = MT * 128 * KST, STAGE = A_BYTES + 128 * KST;   // weights: up to 256 rows
+  static constexpr int NS = MT == 1 ? 6 : 4;
+  // ring, the epilogue warps' staging blocks, alignment of the swizzled tiles
+  static constexpr size_t SMEM = NS * STAGE + PAIR_EPI * 2 * PAIR_BLOCK + 1024;
 };
 constexpr int PAIR_THR = 64 + 32 * PAIR_EPI;
+static_assert(Pair<1>::SMEM + 1280 <= 232448 && Pair<2>::SMEM + 1280 <= 232448, "with the static part, one SM's memory");
 
-// A pair of CTAs (the cluster) works on tiles of 256 tokens x BN weight rows:
-// CTA r holds tokens [128 r, 128 r + 128) and weight rows [BN/2 r, BN/2 (r + 1))
-// of the tile in its shared memory and its tokens' accumulators in its TMEM; CTA
-// 0's warp 1 issues the MMAs of both. With SwiGLU the tile's weight rows are BN/2
-// gate rows (CTA 0's copies) and their up rows (CTA 1's).
-template <int BN>
+// A pair of CTAs (the cluster) works on tiles of 256 MT tokens x bn weight rows
+// (bn a multiple of 32, of 64 with SwiGLU, at most 256): CTA r holds tokens [128 r,
+// 128 r + 128) of each block and weight rows [bn/2 r, bn/2 (r + 1)) of the tile in
+// its shared memory and its tokens' accumulators in its TMEM; CTA 0's warp 1 issues
+// the MMAs of both. With SwiGLU the tile's weight rows are bn/2 gate rows (CTA 0's
+// copies) and their up rows (CTA 1's).
+template <int MT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap ta, Args p, int tiles_m,
-                int tiles, int prefetch, uint64_t timeout) {
-  using L = Pair<BN>;
+    pair_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap ta,
+                const __grid_constant__ CUtensorMap to, Args p, int bn, int tiles_m, int tiles, int prefetch, int tma,
+                uint64_t timeout) {
+  using L = Pair<MT>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[L::NS], empty[L::NS], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem;
-  __shared__ __align__(16) float sws[2][BN];
+  __shared__ __align__(16) float sws[256];              // the tile's weight scales
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int chunks = (p.k + (int)KST - 1) / (int)KST;
-  const int cols = p.swiglu ? BN / 2 : BN;                // output columns of a tile
+  const int cols = p.swiglu ? bn / 2 : bn;                // output columns of a tile
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::NS; ++s) {
@@ -410,14 +433,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * PAIR_EPI);
+      mbar_init(&acc_empty[b], 2 * PAIR_EPI / MT);
     }
     mbar_init(&drained, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem)),
-                 "r"(L::COLS)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -428,10 +450,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
   if (warp == 0 && lane == 0) {
+    const uint32_t bytes = 2 * (L::A_BYTES + (uint32_t)bn / 2 * KST);   // both CTAs' copies of a stage
     auto weights = [&](int tile, int c, int s) {
       const int nt = tile / tiles_m * cols;
-      const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + BN / 2;
-      if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
+      const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + bn / 2;
+      if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
       tma_2d_pair(smem_u32(ring + (size_t)s * L::STAGE) + L::A_BYTES, &tw, c * (int)KST, n0, mapa(smem_u32(&full[s]), 0));
     };
     int ahead = prefetch ? min(L::NS, chunks) : 0;        // stages whose weights are on their way
@@ -440,12 +463,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     int s = 0;
     uint32_t ph = 1;
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
-      const int m0 = tile % tiles_m * 256 + (int)rank * 128;
+      const int m0 = tile % tiles_m * 256 * MT + (int)rank * 128;
       for (int c = 0; c < chunks; ++c) {
         if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
         if (ahead > 0) --ahead;
         else weights(tile, c, s);
-        tma_2d_pair(smem_u32(ring + (size_t)s * L::STAGE), &ta, c * (int)KST, m0, mapa(smem_u32(&full[s]), 0));
+        const uint32_t dst = smem_u32(ring + (size_t)s * L::STAGE), bar = mapa(smem_u32(&full[s]), 0);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) tma_2d_pair(dst + t * 128 * KST, &ta, c * (int)KST, m0 + 256 * t, bar);
         if (++s == L::NS) s = 0, ph ^= 1;
       }
     }
@@ -456,87 +481,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, grace);
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
+    const uint32_t idesc = idesc_i8(256, (uint32_t)bn);
     int s = 0, it = 0;
     uint32_t ph = 0;
     for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
-      const int b = it & 1;
-      if (!(ok = wait_phase(&acc_empty[b], ((it >> 1) & 1) ^ 1, deadline))) break;
-      tc::fence_after_sync();
-      for (int c = 0; c < chunks; ++c) {
-        if (!(ok = wait_phase(&full[s], ph, deadline))) break;
-        tc::fence_after_sync();
-        const uint64_t da = sdesc128(smem_u32(ring + (size_t)s * L::STAGE)), db = da + (L::A_BYTES >> 4);
+      for (int c = 0; ok && c < chunks; ++c) {
+        uint64_t da = 0, db = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma_i8<2>(tmem + (uint32_t)(b * BN), da + 2 * j, db + 2 * j, idesc_i8(256, BN), c > 0 || j > 0);
+        for (int t = 0; t < MT; ++t) {
+          const int b = MT == 1 ? it & 1 : t;             // accumulator
+          if (c == 0) ok = ok && wait_phase(&acc_empty[b], ((MT == 1 ? it >> 1 : it) & 1) ^ 1, deadline);
+          if (t == 0) {
+            ok = ok && wait_phase(&full[s], ph, deadline);
+            da = sdesc128(smem_u32(ring + (size_t)s * L::STAGE));
+            db = da + (L::A_BYTES >> 4);
+          }
+          if (!ok) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_i8<2>(tmem + (uint32_t)(b * 256), da + t * (128 * KST >> 4) + 2 * j, db + 2 * j, idesc, c > 0 || j > 0);
+          if (MT == 2 && t == 0 && c == chunks - 1) commit_pair(&acc_full[0]);
+        }
         commit_pair(&empty[s]);
         if (++s == L::NS) s = 0, ph ^= 1;
       }
-      commit_pair(&acc_full[b]);
+      commit_pair(&acc_full[MT == 1 ? it & 1 : 1]);
     }
     commit_pair(&drained);
     wait_phase(&drained, 0, deadline + timeout);          // no MMA is in flight when TMEM is released
   } else if (warp >= 2) {
-    const int q = warp & 3, et = threadIdx.x - 64;
-    const int osz = p.type == QX_T_F32 ? 4 : 2;
-    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && (p.os * osz) % 16 == 0;
-    uint8_t* stage = ring + L::NS * L::STAGE + (warp - 2) * 32 * PAIR_ROW;
-    const int c_lo = warp >= 6 ? cols / 2 : 0, c_hi = c_lo + cols / 2;
+    const int q = warp & 3, et = threadIdx.x - 64, h = warp >= 6;   // lane quarter, thread, warp group
+    uint8_t* stage = ring + L::NS * L::STAGE + (warp - 2) * 2 * PAIR_BLOCK;
+    int buf = 0;
+    // One block per tile: the two warp groups take alternate pieces of 32 columns;
+    // two blocks: one each.
+    const int block = MT == 1 ? 0 : h, c_lo = MT == 1 ? 32 * h : 0, c_step = MT == 1 ? 64 : 32;
     pdl_wait();                                           // the tokens' scales, and the output's place
-    auto row_of = [&](int tile) { return (int64_t)(tile % tiles_m) * 256 + rank * 128 + q * 32; };
-    // one tile ahead: thread et's weight scale and the lane's token scale
-    auto scale_w = [&](int tile) {
-      const int n = tile / tiles_m * cols + (et < cols ? et : et - cols);
-      return tile < tiles && et < BN && n < p.n ? __ldcg(&p.sw[et < cols ? n : p.n + n]) : 0.f;
+    // The scales one tile ahead: thread et's of a weight row, the lane's of a token.
+    float next_w = 0.f, next_a = 0.f;
+    int64_t next_row = 0;
+    int next_n = 0;
+    auto look_ahead = [&](int tile) {
+      if (tile >= tiles) return;
+      const int tn = tile / tiles_m, n = tn * cols + (et < cols ? et : et - cols);
+      next_n = tn * cols;
+      next_row = (int64_t)(tile - tn * tiles_m) * (256 * MT) + block * 256 + (int)rank * 128 + q * 32;
+      next_w = et < bn && n < p.n ? __ldcg(&p.sw[et < cols ? n : p.n + n]) : 0.f;
+      next_a = next_row + lane < p.m ? __ldcg(&p.sa[next_row + lane]) : 0.f;
     };
-    auto scale_a = [&](int tile) {
-      return tile < tiles && row_of(tile) + lane < p.m ? __ldcg(&p.sa[row_of(tile) + lane]) : 0.f;
-    };
-    float next_w = scale_w(pair), next_a = scale_a(pair);
+    look_ahead(pair);
     int it = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++it) {
-      const int b = it & 1;
-      const int n0 = tile / tiles_m * cols;
-      const int64_t row0 = row_of(tile);
+      const int b = MT == 1 ? it & 1 : h;                 // accumulator
+      const int n0 = next_n;
+      const int64_t row0 = next_row;
       const float sa = next_a;
-      if (et < BN) sws[b][et] = next_w;
-      next_w = scale_w(tile + pairs);
-      next_a = scale_a(tile + pairs);
-      ok = wait_phase(&acc_full[b], (it >> 1) & 1, deadline);
-      if (!epilogue_and(ok)) break;                       // also: sws of this tile is written
+      asm volatile("bar.sync 1, 256;" ::: "memory");      // the last tile's sws have been read
+      sws[et] = next_w;
+      look_ahead(tile + pairs);
+      if (!epilogue_and(ok)) break;                       // this tile's sws are written; a wait that ran out ends all
+      ok = __all_sync(0xffffffffu, wait_phase(&acc_full[b], (MT == 1 ? it >> 1 : it) & 1, deadline));
+      if (!ok) continue;
       tc::fence_after_sync();
-      const uint32_t t0 = tmem + (uint32_t)(b * BN) + ((uint32_t)(q * 32) << 16);
+      const uint32_t t0 = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-      for (int c = c_lo; c < c_hi && n0 + c < p.n; c += 32) {
+      for (int c = c_lo; c < cols && n0 + c < p.n; c += c_step) {
         int32_t g[32];
         float v[32];
         tm_ld32(t0 + c, g);
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          const float2 r = scaled2(g[j], g[j + 1], sa, *reinterpret_cast<const float2*>(&sws[b][c + j]));
+          const float2 r = scaled2(g[j], g[j + 1], sa, *reinterpret_cast<const float2*>(sws + c + j));
           v[j] = r.x;
           v[j + 1] = r.y;
         }
         if (p.swiglu) {
-          tm_ld32(t0 + BN / 2 + c, g);
+          tm_ld32(t0 + cols + c, g);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float2 r = scaled2(g[j], g[j + 1], sa, *reinterpret_cast<const float2*>(&sws[b][BN / 2 + c + j]));
+            const float2 r = scaled2(g[j], g[j + 1], sa, *reinterpret_cast<const float2*>(sws + cols + c + j));
             v[j] = swiglu(v[j], r.x, p.limit, p.has_limit);
             v[j + 1] = swiglu(v[j + 1], r.y, p.limit, p.has_limit);
           }
         }
-        if (row0 < p.m) store_block(p, stage, row0, n0 + c, v, vec, lane);
+        if (row0 >= p.m) continue;
+        if (p.type != QX_T_F32) {
+          store_block<32>(p, &to, stage + buf * PAIR_BLOCK, row0, n0 + c, v, tma, lane);
+          buf ^= 1;
+        } else {
+          store_block<16>(p, &to, stage + buf * PAIR_BLOCK, row0, n0 + c, v, tma, lane);
+          if (n0 + c + 16 < p.n) store_block<16>(p, &to, stage + (buf ^ 1) * PAIR_BLOCK, row0, n0 + c + 16, v + 16, tma, lane);
+          else buf ^= 1;
+        }
       }
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_cluster(mapa(smem_u32(&acc_empty[b]), 0));
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the stores are in memory
   }
   __syncwarp();
   tc::fence_before_sync();
   cluster_sync();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::COLS) : "memory");
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace i8

@@ -136,7 +136,8 @@ def test_quantiser_fp8_rows_and_strides(cuda_ready):
 
 SIZES = [(1, 1, 1), (1, 8, 16), (1, 4608, 512), (2, 131, 130), (16, 128, 128), (17, 129, 257), (37, 1003, 2311),
          (64, 64, 5120), (65, 320, 96), (128, 256, 384), (129, 257, 129), (200, 640, 1000), (300, 72, 2304),
-         (513, 515, 300), (1025, 384, 160)]
+         (513, 515, 300), (1025, 384, 160),
+         (1024, 5120, 272), (2100, 640, 208), (700, 9000, 64), (3000, 301, 130), (4500, 2304, 96)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -173,7 +174,7 @@ def test_matmul_largest_sums(cuda_ready):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 2304, 512), (6, 100, 5120), (33, 65, 300), (130, 128, 128),
-                                   (257, 333, 1111), (600, 384, 640)])
+                                   (257, 333, 1111), (600, 384, 640), (1500, 2304, 144), (4100, 1111, 96)])
 @pytest.mark.parametrize("limit", [10.0, 0.5, 0.0])
 @pytest.mark.parametrize("pad", [True, False])
 def test_swiglu(cuda_ready, m, n, k, limit, pad):

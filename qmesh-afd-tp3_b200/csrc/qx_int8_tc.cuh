@@ -49,6 +49,15 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
         : "memory");
 }
 
+// One lane of a converged warp, chosen so that the compiler knows it is one: the
+// copies and MMAs of a lane picked by its number go through a loop over the
+// active lanes (about 80 cycles each).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0u;
+}
+
 // ---- TMA, clusters ----------------------------------------------------------------
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -152,8 +161,9 @@ __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
 
 // ------------------------------------------------------------------ few tokens
 // Grid: (row tile of 128 weight rows, token tile of BN tokens, K piece), the K
-// pieces of one tile in one cluster. Warp 0 copies, warp 1 issues the MMAs, warps
-// 2-5 bring the accumulator to shared memory; then every CTA of the cluster adds
+// pieces of one tile in one cluster. Warps 0 and 6 copy weights and tokens (one
+// thread's copies for both took longer than their flight), warp 1 issues the MMAs,
+// warps 2-5 bring the accumulator to shared memory; then every CTA of the cluster adds
 // a share of the tile over the pieces and writes it. With SwiGLU the 128 rows are
 // 64 gate rows and their 64 up rows. The ring is small enough for two CTAs per SM.
 template <int BN>
@@ -164,7 +174,7 @@ struct Split {
   static constexpr size_t SMEM = NS * STAGE + 1024;      // 1024: alignment of the swizzled tiles
   static_assert(BN * 128 * 4 <= NS * STAGE, "the accumulator fits the drained ring");
 };
-constexpr int SPLIT_THR = 192;
+constexpr int SPLIT_THR = 224;
 
 template <int BN>
 __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant__ CUtensorMap tw,
@@ -200,29 +210,34 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   tc::fence_after_sync();
   const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
-  if (warp == 0 && lane == 0) {
-    auto weights = [&](int c, int s) {
-      const uint32_t dst = smem_u32(ring + (size_t)s * L::STAGE), bar = smem_u32(&full[s]);
-      mbar_arrive_expect_tx(&full[s], L::STAGE);
-      tma_2d(dst, &tw, c * (int)KST, n0, bar);
-      tma_2d(dst + 64 * KST, &tw, c * (int)KST, p.swiglu ? p.n + n0 : n0 + 64, bar);
-    };
-    const int ahead = prefetch ? min(L::NS, c1 - c0) : 0;
-    for (int s = 0; s < ahead; ++s) weights(c0 + s, s);
-    pdl_wait();
+  if (warp == 0 && elect_one()) {
+    if (!prefetch) pdl_wait();
+    const uint32_t base = smem_u32(ring), bars = smem_u32(full);
+    const int n1 = p.swiglu ? p.n + n0 : n0 + 64;          // the tile's second 64 rows
     int s = 0;
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
-      if (c - c0 >= ahead) weights(c, s);
-      tma_2d(smem_u32(ring + (size_t)s * L::STAGE) + L::A_BYTES, &ta, c * (int)KST, m0, smem_u32(&full[s]));
+      mbar_arrive_expect_tx(&full[s], L::STAGE);
+      tma_2d(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
+      tma_2d(base + s * L::STAGE + 64 * KST, &tw, c * (int)KST, n1, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
     if (!ok) {                                            // copies still in flight land before the CTA leaves
       const uint64_t grace = globaltimer_ns() + timeout;
       for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, grace);
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 6 && elect_one()) {
+    pdl_wait();
+    const uint32_t base = smem_u32(ring) + L::A_BYTES, bars = smem_u32(full);
+    int s = 0;
+    uint32_t ph = 1;
+    for (int c = c0; c < c1; ++c) {
+      if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+      tma_2d(base + s * L::STAGE, &ta, c * (int)KST, m0, bars + 8 * s);
+      if (++s == L::NS) s = 0, ph ^= 1;
+    }
+  } else if (warp == 1 && elect_one()) {
     int s = 0;
     uint32_t ph = 0;
     for (int c = c0; c < c1; ++c) {
@@ -239,7 +254,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   __syncwarp();
   const int cols = min(BN, p.m - m0);                     // tokens of the tile
   int32_t* red = reinterpret_cast<int32_t*>(ring);        // [token][128 weight rows]
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     ok = wait_phase(&done, 0, deadline + timeout);
     tc::fence_after_sync();
     if (__all_sync(0xffffffffu, ok)) {
@@ -400,7 +415,7 @@ struct Pair {
   // ring, the epilogue warps' staging blocks, alignment of the swizzled tiles
   static constexpr size_t SMEM = NS * STAGE + PAIR_EPI * 2 * PAIR_BLOCK + 1024;
 };
-constexpr int PAIR_THR = 64 + 32 * PAIR_EPI;
+constexpr int PAIR_THR = 96 + 32 * PAIR_EPI;         // weight copies, MMAs, epilogue, token copies
 static_assert(Pair<1>::SMEM + 1280 <= 232448 && Pair<2>::SMEM + 1280 <= 232448, "with the static part, one SM's memory");
 
 // A pair of CTAs (the cluster) works on tiles of 256 MT tokens x bn weight rows
@@ -449,28 +464,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   tc::fence_after_sync();
   const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
-  if (warp == 0 && lane == 0) {
+  if (warp == 0 && elect_one()) {
     const uint32_t bytes = 2 * (L::A_BYTES + (uint32_t)bn / 2 * KST);   // both CTAs' copies of a stage
-    auto weights = [&](int tile, int c, int s) {
-      const int nt = tile / tiles_m * cols;
-      const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + bn / 2;
-      if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-      tma_2d_pair(smem_u32(ring + (size_t)s * L::STAGE) + L::A_BYTES, &tw, c * (int)KST, n0, mapa(smem_u32(&full[s]), 0));
-    };
-    int ahead = prefetch ? min(L::NS, chunks) : 0;        // stages whose weights are on their way
-    for (int s = 0; s < ahead; ++s) weights(pair, s, s);
-    pdl_wait();
+    // Weights (and CTA 0's count of both CTAs' bytes of a stage). Weights that are
+    // complete already need not wait for the kernel in front.
+    if (!prefetch) pdl_wait();
+    const uint32_t base = smem_u32(ring) + L::A_BYTES, bars = mapa(smem_u32(full), 0);
     int s = 0;
     uint32_t ph = 1;
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
-      const int m0 = tile % tiles_m * 256 * MT + (int)rank * 128;
+      const int nt = tile / tiles_m * cols;
+      const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + bn / 2;
       for (int c = 0; c < chunks; ++c) {
         if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
-        if (ahead > 0) --ahead;
-        else weights(tile, c, s);
-        const uint32_t dst = smem_u32(ring + (size_t)s * L::STAGE), bar = mapa(smem_u32(&full[s]), 0);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) tma_2d_pair(dst + t * 128 * KST, &ta, c * (int)KST, m0 + 256 * t, bar);
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+        tma_2d_pair(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
         if (++s == L::NS) s = 0, ph ^= 1;
       }
     }
@@ -480,7 +488,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       const uint64_t grace = globaltimer_ns() + timeout;
       for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, grace);
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 2 + PAIR_EPI && elect_one()) {
+    pdl_wait();
+    const uint32_t base = smem_u32(ring), bars = mapa(smem_u32(full), 0);
+    int s = 0;
+    uint32_t ph = 1;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      const int m0 = tile % tiles_m * 256 * MT + (int)rank * 128;
+      for (int c = 0; c < chunks; ++c) {
+        if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          tma_2d_pair(base + s * L::STAGE + t * 128 * KST, &ta, c * (int)KST, m0 + 256 * t, bars + 8 * s);
+        if (++s == L::NS) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1 && rank == 0 && elect_one()) {
     const uint32_t idesc = idesc_i8(256, (uint32_t)bn);
     int s = 0, it = 0;
     uint32_t ph = 0;
@@ -510,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     }
     commit_pair(&drained);
     wait_phase(&drained, 0, deadline + timeout);          // no MMA is in flight when TMEM is released
-  } else if (warp >= 2) {
+  } else if (warp >= 2 && warp < 2 + PAIR_EPI) {
     const int q = warp & 3, et = threadIdx.x - 64, h = warp >= 6;   // lane quarter, thread, warp group
     uint8_t* stage = ring + L::NS * L::STAGE + (warp - 2) * 2 * PAIR_BLOCK;
     int buf = 0;

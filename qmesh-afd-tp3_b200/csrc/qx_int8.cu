@@ -297,10 +297,7 @@ int device_sms() {
   const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
   if (cudaFuncSetAttribute(split_kernel<16>, attr, (int)Split<16>::SMEM) != cudaSuccess ||
       cudaFuncSetAttribute(split_kernel<32>, attr, (int)Split<32>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(split_kernel<64>, attr, (int)Split<64>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(split_kernel<128>, attr, (int)Split<128>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(pair_kernel<1>, attr, (int)Pair<1>::SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(pair_kernel<2>, attr, (int)Pair<2>::SMEM) != cudaSuccess)
+      cudaFuncSetAttribute(pair_kernel, attr, (int)PAIR_SMEM) != cudaSuccess)
     return 0;
   return cached[dev] = sms;
 }
@@ -365,85 +362,68 @@ struct Launch {
   }
 };
 
-template <int BN>
-int split_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, int pieces, int prefetch,
-                 cudaStream_t st) {
-  const int half = p.swiglu ? 64 : 128;
-  const dim3 grid((unsigned)((p.n + half - 1) / half * pieces), (unsigned)((p.m + BN - 1) / BN), 1);
-  return Launch(grid, SPLIT_THR, Split<BN>::SMEM, st, pieces)(split_kernel<BN>, tw, ta, p, pieces, prefetch,
-                                                            wait_limit_ns());
-}
-
-// Tile of the pair kernel: 256 mt tokens x bn weight rows.
-struct PairTile {
-  int mt, bn, tiles_m;
-  int64_t tiles;
-};
-
-// The tile with the smallest estimated time: waves of tiles over the pairs, each
-// 128-byte chunk of K taking the longer of its MMAs (335 ns for 256 x 256, measured
-// without copies) and its copies (both CTAs' operands of every busy pair at 11.5
-// TB/s, measured), and an epilogue (1.4 us for 256 x 256) that only one block per
-// tile hides, but for the last.
-PairTile pair_tile(const Args& p, int sms) {
-  const int pairs = sms / 2, chunks = (p.k + (int)KST - 1) / (int)KST, h = p.swiglu ? 2 : 1, step = 32 * h;
-  PairTile best = {};
+// Tile of the pair kernel: tokens per CTA (the tokens spread evenly over the fewest
+// tiles of 256) and the weight rows with the smallest estimated time. A wave of tiles
+// over the pairs takes, per 128-byte chunk of K, the longer of the MMAs (1.3 ns a weight
+// row) and the copies into one SM (64 bytes a clock: 1.05 ns a row of its operands, 60 ns
+// at least), or an epilogue (1.4 us for 256 rows) if that is longer; the last epilogue
+// comes on top. Measured at 2048 x 5120 x 2304: 18.3 us with 192 rows (3 waves), 20.8 with
+// 256 (3), 22.8 with 128 (5).
+void pair_tile(const Args& p, int sms, int* tb, int* bn) {
+  const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, chunks = (p.k + (int)KST - 1) / (int)KST;
+  const int h = p.swiglu ? 2 : 1, step = 32 * h;
+  *tb = (p.m + 16 * tiles_m - 1) / (16 * tiles_m) * 8;
   double least = 0;
-  for (int mt = 1; mt <= 2; ++mt) {
-    for (int bn = 2 * step; bn <= 256; bn += step) {
-      PairTile t = {mt, bn, (p.m + 256 * mt - 1) / (256 * mt), 0};
-      t.tiles = (int64_t)t.tiles_m * ((p.n + bn / h - 1) / (bn / h));
-      const double waves = (double)((t.tiles + pairs - 1) / pairs), busy = (double)(t.tiles < pairs ? t.tiles : pairs);
-      const double mma = 335.0 * mt * bn / 256, copy = (mt * 16384 + bn * 64) * 2 * busy / 11500.0;
-      const double epi = 1400.0 * bn / 256, loop = chunks * (mma > copy ? mma : copy);
-      const double ns = mt == 1 ? waves * (loop > epi ? loop : epi) + epi : waves * (loop + epi);
-      if (best.mt == 0 || ns < least) best = t, least = ns;
-    }
+  for (int b = 256; b >= 64; b -= step) {
+    const int64_t tiles = (int64_t)tiles_m * ((p.n + b / h - 1) / (b / h));
+    const double mma = 1.3 * b, copy = 1.05 * (*tb + b / 2), epi = 1400.0 * b / 256;
+    const double chunk = mma > copy ? (mma > 60 ? mma : 60) : (copy > 60 ? copy : 60), loop = chunks * chunk;
+    const double ns = (double)((tiles + pairs - 1) / pairs) * (loop > epi ? loop : epi) + epi;
+    if (least == 0 || ns < least) *bn = b, least = ns;
   }
-  return best;
 }
 
-template <int MT>
-int pair_launch(const Args& p, const CUtensorMap& tw, const CUtensorMap& ta, const PairTile& t, int prefetch, int sms,
-                cudaStream_t st) {
-  if (t.tiles > 0x7fffffff) return QX_ERR_SHAPE;
-  const int pairs = (int)(t.tiles < sms / 2 ? t.tiles : sms / 2), osz = element_size(p.type);
-  // Tiled stores where the output's rows start on 16-byte boundaries.
-  CUtensorMap to = {};
-  const int tma = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.os * osz % 16 == 0 &&
-                  tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-  return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, Pair<MT>::SMEM, st, 2)(pair_kernel<MT>, tw, ta, to, p, t.bn, t.tiles_m,
-                                                                       (int)t.tiles, prefetch, tma, wait_limit_ns());
+int pair_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
+  int tb = 0, bn = 0;
+  pair_tile(p, sms, &tb, &bn);
+  const int cols = p.swiglu ? bn / 2 : bn, tiles_m = (p.m + 2 * tb - 1) / (2 * tb);
+  const int64_t tiles = (int64_t)tiles_m * ((p.n + cols - 1) / cols);
+  if (tiles > 0x7fffffff) return QX_ERR_SHAPE;
+  const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2), osz = element_size(p.type);
+  CUtensorMap tw, ta, to = {};
+  if (!row_map(&tw, p.w, p.swiglu ? 2ll * p.n : p.n, p.k, p.ws, bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, tb))
+    return QX_ERR_DEVICE;
+  const int spans = bn >= 160 ? 1 : 2;   // from 160 rows on the MMAs of one span outlast the issuing threads' loop
+  // Tiled stores where the output's rows start on 16-byte boundaries, in boxes that do
+  // not reach from a CTA's tokens into the next one's.
+  int tma = tb % 32 ? 8 : 32;
+  if (reinterpret_cast<uintptr_t>(p.out) % 16 || p.os * osz % 16 ||
+      !tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, tma, CU_TENSOR_MAP_SWIZZLE_64B))
+    tma = 0;
+  return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, PAIR_SMEM, st, 2)(pair_kernel, tw, ta, to, p, tb, bn, spans, tiles_m,
+                                                                  (int)tiles, prefetch, tma, wait_limit_ns());
 }
 
-// K pieces of the split kernel: the count (1..8) that leaves the busiest SM the
-// fewest K chunks, the smallest of equals.
-int pieces_of(int tiles, int chunks, int sms) {
+// K pieces of the split kernel (1..8, at most one per stage of K): the fewest that
+// leave a CTA the least of K while all clusters fit on the GPU at once (two CTAs per
+// SM, less what clusters leave unused of a group of SMs: 1.65 per SM).
+int pieces_of(int64_t tiles, int stages, int sms) {
   int best = 1;
-  int64_t least = -1;
-  for (int s = 1; s <= 8 && s <= chunks; ++s) {
-    const int64_t c = (int64_t)((int64_t)tiles * s + sms - 1) / sms * ((chunks + s - 1) / s);
-    if (least < 0 || c < least) best = s, least = c;
-  }
+  for (int s = 2; s <= 8 && s <= stages; ++s)
+    if (tiles * s * 20 <= (int64_t)sms * 33 && (stages + s - 1) / s < (stages + best - 1) / best) best = s;
   return best;
 }
 
-int tc_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
+template <int BN>
+int split_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
+  using L = Split<BN>;
+  const int half = p.swiglu ? 64 : 128, tiles_n = (p.n + half - 1) / half, tiles_m = (p.m + BN - 1) / BN;
+  const int pieces = pieces_of((int64_t)tiles_n * tiles_m, (p.k + (int)KSTAGE - 1) / (int)KSTAGE, sms);
   CUtensorMap tw, ta;
-  const int64_t w_rows = p.swiglu ? 2ll * p.n : p.n;
-  if (p.m <= 128) {
-    const int bn = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-    if (!row_map(&tw, p.w, w_rows, p.k, p.ws, 64) || !row_map(&ta, p.a, p.m, p.k, p.as, bn)) return QX_ERR_DEVICE;
-    const int half = p.swiglu ? 64 : 128;
-    const int s = pieces_of((p.n + half - 1) / half, (p.k + (int)KST - 1) / (int)KST, sms);
-    return bn == 16   ? split_launch<16>(p, tw, ta, s, prefetch, st)
-           : bn == 32 ? split_launch<32>(p, tw, ta, s, prefetch, st)
-           : bn == 64 ? split_launch<64>(p, tw, ta, s, prefetch, st)
-                      : split_launch<128>(p, tw, ta, s, prefetch, st);
-  }
-  const PairTile t = pair_tile(p, sms);
-  if (!row_map(&tw, p.w, w_rows, p.k, p.ws, t.bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, 128)) return QX_ERR_DEVICE;
-  return t.mt == 1 ? pair_launch<1>(p, tw, ta, t, prefetch, sms, st) : pair_launch<2>(p, tw, ta, t, prefetch, sms, st);
+  if (!row_map(&tw, p.w, p.swiglu ? 2ll * p.n : p.n, p.k, p.ws, half) || !row_map(&ta, p.a, p.m, p.k, p.as, BN))
+    return QX_ERR_DEVICE;
+  return Launch(dim3((unsigned)(tiles_n * pieces), (unsigned)tiles_m, 1), SPLIT_THR, L::SMEM, st, pieces)(
+      split_kernel<BN>, tw, ta, p, pieces, prefetch, wait_limit_ns());
 }
 
 // A checked product. prefetch: the weights are complete when this kernel starts,
@@ -456,7 +436,10 @@ int product(Args p, int prefetch, int sms, cudaStream_t st) {
   if (aligned(p.a, p.as, p.m) && aligned(p.w, p.ws, p.swiglu ? 2 : p.n)) {
     if (p.m == 1) p.as = (p.as + 15) / 16 * 16;          // never stepped
     if (p.n == 1 && !p.swiglu) p.ws = (p.ws + 15) / 16 * 16;
-    return tc_launch(p, prefetch, sms, st);
+    // Up to 32 tokens by K pieces, more by pairs (4608 x 5120: 8.2 us against 9.0 with 1
+    // token, 9.4 against 9.1 with 32, 11.7 against 9.0 with 64).
+    if (p.m > 32) return pair_launch(p, prefetch, sms, st);
+    return p.m <= 16 ? split_launch<16>(p, prefetch, sms, st) : split_launch<32>(p, prefetch, sms, st);
   }
   const int half = p.swiglu ? ST / 2 : ST;
   const int64_t gy = (p.m + ST - 1) / ST;

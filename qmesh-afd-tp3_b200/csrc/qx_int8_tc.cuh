@@ -1,14 +1,14 @@
 // Tensor-core kernels of the int8 product (tcgen05.mma.kind::i8, int8 x int8
 // into int32 accumulators in TMEM), operands brought in by tiled TMA copies with
-// the 128-byte swizzle: one stage of the shared-memory ring is 128 bytes of K of
-// an operand tile's rows, four MMAs of K = 32.
+// the 128-byte swizzle: a stage of the shared-memory ring is 256 bytes of K of the
+// operand tiles' rows, eight MMAs of K = 32.
 //
 //   split_kernel  few tokens: weights are the M = 128 operand, tokens the N
 //                 operand, and the CTAs of a cluster split K (their sums, whole
 //                 numbers, meet over distributed shared memory).
 //   pair_kernel   many tokens: persistent pairs of CTAs (cta_group::2), 256
-//                 tokens x BN weight rows per tile, two accumulators so that one
-//                 tile's epilogue runs under the next one's MMAs.
+//                 tokens x up to 256 weight rows per tile, two accumulators so that
+//                 one tile's epilogue runs under the next one's MMAs.
 #pragma once
 
 #include <cuda.h>
@@ -18,7 +18,10 @@
 namespace qx {
 namespace i8 {
 
-constexpr uint32_t KST = 128;            // K bytes per stage (one swizzle span)
+// One swizzle span of K per tiled copy. A stage of a ring holds two of them (large
+// tiles of the pair kernel: one), so that the issuing threads' waits and loop, about
+// 300 cycles, are paid once per 256 bytes of K. K past the end reads as 0.
+constexpr uint32_t KST = 128, KSTAGE = 2 * KST;
 
 // ---- descriptors -----------------------------------------------------------------
 // Shared-memory descriptor of a K-major tile with the 128-byte swizzle: rows 128
@@ -86,6 +89,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The barrier in two halves and without memory order: nothing that was written before
+// it is read after it, and the ordered form would wait for the global stores (2 us).
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
@@ -108,22 +120,28 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       : "memory");
 }
 
-// Bounded wait: false once the deadline has passed, with
-// QX_DEV_TIMEOUT recorded; the caller then stops consuming.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint64_t deadline) {
+__device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0u;
+}
+
+// Bounded wait: false once the deadline has passed, with QX_DEV_TIMEOUT recorded;
+// the caller then stops consuming.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t deadline) {
   for (uint32_t it = 0;; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
+    if (try_phase(bar, parity)) return true;
     if ((it & 15u) == 15u && globaltimer_ns() > deadline) {
       atomicOr(&g_status, (uint32_t)QX_DEV_TIMEOUT);
       return false;
     }
   }
+}
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint64_t deadline) {
+  return try_phase(bar, parity) || wait_long(bar, parity, deadline);
 }
 
 // ---- accumulator loads ---------------------------------------------------------------
@@ -165,13 +183,15 @@ __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
 // thread's copies for both took longer than their flight), warp 1 issues the MMAs,
 // warps 2-5 bring the accumulator to shared memory; then every CTA of the cluster adds
 // a share of the tile over the pieces and writes it. With SwiGLU the 128 rows are
-// 64 gate rows and their 64 up rows. The ring is small enough for two CTAs per SM.
+// 64 gate rows and their 64 up rows. The ring takes
+// half an SM, so that two CTAs run side by side.
 template <int BN>
 struct Split {
-  static constexpr uint32_t A_BYTES = 128 * KST, B_BYTES = BN * KST, STAGE = A_BYTES + B_BYTES;
-  static constexpr int NS = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
+  // a stage: two spans of 128 weight rows, then two of BN token rows
+  static constexpr uint32_t A_SPAN = 128 * KST, B_SPAN = BN * KST, A_BYTES = 2 * A_SPAN, STAGE = A_BYTES + 2 * B_SPAN;
   static constexpr uint32_t COLS = BN < 32 ? 32 : BN;
-  static constexpr size_t SMEM = NS * STAGE + 1024;      // 1024: alignment of the swizzled tiles
+  static constexpr int NS = 114688 / STAGE;              // two CTAs per SM
+  static constexpr size_t SMEM = (size_t)NS * STAGE + 1024;   // 1024: alignment of the swizzled tiles
   static_assert(BN * 128 * 4 <= NS * STAGE, "the accumulator fits the drained ring");
 };
 constexpr int SPLIT_THR = 224;
@@ -189,10 +209,12 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   const int rank = pieces > 1 ? (int)cluster_rank() : 0;
   const int half = p.swiglu ? 64 : 128;                  // output columns of a tile
   const int n0 = (int)(blockIdx.x / pieces) * half, m0 = blockIdx.y * BN;
-  const int chunks = (p.k + (int)KST - 1) / (int)KST;
+  const int chunks = (p.k + (int)KSTAGE - 1) / (int)KSTAGE;
   const int c0 = (int)((int64_t)chunks * rank / pieces), c1 = (int)((int64_t)chunks * (rank + 1) / pieces);
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
+    prefetch_map(&tw);
+    prefetch_map(&ta);
     for (int s = 0; s < L::NS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -213,14 +235,18 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   if (warp == 0 && elect_one()) {
     if (!prefetch) pdl_wait();
     const uint32_t base = smem_u32(ring), bars = smem_u32(full);
-    const int n1 = p.swiglu ? p.n + n0 : n0 + 64;          // the tile's second 64 rows
     int s = 0;
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
       mbar_arrive_expect_tx(&full[s], L::STAGE);
-      tma_2d(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
-      tma_2d(base + s * L::STAGE + 64 * KST, &tw, c * (int)KST, n1, bars + 8 * s);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = c * (int)KSTAGE + h * (int)KST;
+        const uint32_t to = base + s * L::STAGE + h * L::A_SPAN;
+        tma_2d(to, &tw, k, n0, bars + 8 * s);
+        if (p.swiglu) tma_2d(to + 64 * KST, &tw, k, p.n + n0, bars + 8 * s);
+      }
       if (++s == L::NS) s = 0, ph ^= 1;
     }
     if (!ok) {                                            // copies still in flight land before the CTA leaves
@@ -234,7 +260,9 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
-      tma_2d(base + s * L::STAGE, &ta, c * (int)KST, m0, bars + 8 * s);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        tma_2d(base + s * L::STAGE + h * L::B_SPAN, &ta, c * (int)KSTAGE + h * (int)KST, m0, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
   } else if (warp == 1 && elect_one()) {
@@ -245,7 +273,9 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       tc::fence_after_sync();
       const uint64_t da = sdesc128(smem_u32(ring + (size_t)s * L::STAGE)), db = da + (L::A_BYTES >> 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_i8<1>(tmem, da + 2 * j, db + 2 * j, idesc_i8(128, BN), c > c0 || j > 0);
+      for (int j = 0; j < 8; ++j)
+        mma_i8<1>(tmem, da + (j >> 2) * (L::A_SPAN >> 4) + 2 * (j & 3), db + (j >> 2) * (L::B_SPAN >> 4) + 2 * (j & 3),
+                  idesc_i8(128, BN), c > c0 || j > 0);
       tc::commit(&empty[s]);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
@@ -318,7 +348,12 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
         if (n + j < p.n) store_out(p.out, at + j, p.type, v[j]);
     }
   }
-  if (pieces > 1) cluster_sync(); else __syncthreads();   // the others have read this CTA's sums
+  // No CTA leaves before the others have read its sums.
+  __syncwarp();
+  if (pieces > 1) {
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   if (warp == 1) tc::tmem_dealloc(tmem, L::COLS);
 }
 
@@ -340,12 +375,13 @@ __device__ __forceinline__ bool epilogue_and(bool pred) {
 // different banks. Two buffers, so that a store drains while the next block is written.
 constexpr int PAIR_BLOCK = 32 * 64;
 
-// 32 tokens x COLS output columns from column n on, each lane holding its token's
-// values. Rows on 16-byte boundaries (tma): one tiled store, which leaves out what
-// lies past the tensor's end; else element by element, 64 bytes of a row at a time.
+// Up to 32 tokens (rows) x COLS output columns from column n on, each lane holding its
+// token's values. Rows on 16-byte boundaries: tiled stores of `tma` (8 or 32) tokens,
+// which leave out what lies past the tensor's end; else (tma = 0) element by element,
+// 64 bytes of a row at a time.
 template <int COLS>
-__device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to, uint8_t* stage, int64_t row0, int n,
-                                            const float* v, bool tma, int lane) {
+__device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to, uint8_t* stage, int64_t row0, int rows,
+                                            int n, const float* v, int tma, int lane) {
   constexpr int OSZ = 64 / COLS;
   uint8_t* mine = stage + lane * 64;
   const int sw = (lane >> 1) & 3;
@@ -366,20 +402,21 @@ __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) {
-      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(to), "r"(n),
-                   "r"((int)row0), "r"(smem_u32(stage))
-                   : "memory");
+      for (int r = 0; r < min(rows, 32); r += tma)
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(to), "r"(n),
+                     "r"((int)row0 + r), "r"(smem_u32(stage) + r * 64)
+                     : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     return;
   }
   __syncwarp();
-  const int rows = (int)min((int64_t)32, p.m - row0), c = lane % COLS;
+  const int c = lane % COLS;
   const int64_t step = p.os * OSZ;
   uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + row0 * step + (int64_t)(n + c) * OSZ;
   if (n + c < p.n) {
 #pragma unroll 4
-    for (int r = lane / COLS; r < rows; r += 32 / COLS) {
+    for (int r = lane / COLS; r < min(rows, 32); r += 32 / COLS) {
       const uint8_t* from = stage + r * 64 + 16 * ((c * OSZ / 16) ^ ((r >> 1) & 3)) + c * OSZ % 16;
       if constexpr (OSZ == 4) *reinterpret_cast<float*>(out + r * step) = *reinterpret_cast<const float*>(from);
       else *reinterpret_cast<uint16_t*>(out + r * step) = *reinterpret_cast<const uint16_t*>(from);
@@ -405,50 +442,53 @@ __device__ __forceinline__ float2 scaled2(int32_t a, int32_t b, float sa, float2
   return r;
 }
 
-// MT: 256-token blocks per tile. One block leaves room for two accumulators, so a
-// tile's epilogue runs under the next one's MMAs; two blocks share every weight
-// copy, which brings the copies below the MMAs' time, with no second accumulator.
-template <int MT>
-struct Pair {
-  static constexpr uint32_t A_BYTES = MT * 128 * KST, STAGE = A_BYTES + 128 * KST;   // weights: up to 256 rows
-  static constexpr int NS = MT == 1 ? 6 : 4;
-  // ring, the epilogue warps' staging blocks, alignment of the swizzled tiles
-  static constexpr size_t SMEM = NS * STAGE + PAIR_EPI * 2 * PAIR_BLOCK + 1024;
-};
+constexpr size_t PAIR_RING = 196608;
+constexpr int MAX_NS = 12;               // stages of the pair kernel's ring at most
+// ring, the epilogue warps' staging blocks, alignment of the swizzled tiles
+constexpr size_t PAIR_SMEM = PAIR_RING + PAIR_EPI * 2 * PAIR_BLOCK + 1024;
 constexpr int PAIR_THR = 96 + 32 * PAIR_EPI;         // weight copies, MMAs, epilogue, token copies
-static_assert(Pair<1>::SMEM + 1280 <= 232448 && Pair<2>::SMEM + 1280 <= 232448, "with the static part, one SM's memory");
+static_assert(PAIR_SMEM + 1536 <= 232448, "with the static part, one SM's memory");
 
-// A pair of CTAs (the cluster) works on tiles of 256 MT tokens x bn weight rows
-// (bn a multiple of 32, of 64 with SwiGLU, at most 256): CTA r holds tokens [128 r,
-// 128 r + 128) of each block and weight rows [bn/2 r, bn/2 (r + 1)) of the tile in
-// its shared memory and its tokens' accumulators in its TMEM; CTA 0's warp 1 issues
-// the MMAs of both. With SwiGLU the tile's weight rows are bn/2 gate rows (CTA 0's
-// copies) and their up rows (CTA 1's).
-template <int MT>
+// A pair of CTAs (the cluster) works on tiles of 2 tb tokens x bn weight rows (tb a
+// multiple of 8, at most 128; bn a multiple of 32, of 64 with SwiGLU, at most 256):
+// CTA r holds tokens [tb r, tb (r + 1)) and weight rows [bn/2 r, bn/2 (r + 1)) of the
+// tile in its shared memory and its tokens' accumulators in its TMEM; CTA 0's warp 1
+// issues the MMAs of both (always M = 256: the rows from tb on read whatever follows
+// in shared memory and are not used). With SwiGLU the tile's weight rows are bn/2 gate
+// rows (CTA 0's copies) and their up rows (CTA 1's). The ring holds as many stages as
+// fit (6 of one span for tb = 128, bn = 256). Tiles of 512 tokens (every weight copy used twice, one
+// accumulator per block) were slower from 2048 tokens up: their epilogues run alone,
+// and all at once.
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap ta,
-                const __grid_constant__ CUtensorMap to, Args p, int bn, int tiles_m, int tiles, int prefetch, int tma,
-                uint64_t timeout) {
-  using L = Pair<MT>;
+                const __grid_constant__ CUtensorMap to, Args p, int tb, int bn, int spans, int tiles_m, int tiles,
+                int prefetch, int tma, uint64_t timeout) {
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[L::NS], empty[L::NS], acc_full[2], acc_empty[2], drained;
+  __shared__ uint64_t full[MAX_NS], empty[MAX_NS], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem;
   __shared__ __align__(16) float sws[256];              // the tile's weight scales
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int chunks = (p.k + (int)KST - 1) / (int)KST;
+  const int kst = spans * (int)KST, stages = (p.k + kst - 1) / kst;   // K of a stage, stages of a tile
   const int cols = p.swiglu ? bn / 2 : bn;                // output columns of a tile
+  // a stage: its spans of the tokens, then of the weight rows
+  const uint32_t a_span = (uint32_t)tb * KST, b_span = (uint32_t)bn / 2 * KST;
+  const uint32_t stage_bytes = spans * (a_span + b_span);
+  const int ns = min(MAX_NS, (int)(PAIR_RING / stage_bytes));
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L::NS; ++s) {
+    prefetch_map(&tw);
+    prefetch_map(&ta);
+    if (tma) prefetch_map(&to);
+    for (int s = 0; s < ns; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * PAIR_EPI / MT);
+      mbar_init(&acc_empty[b], 2 * PAIR_EPI);
     }
     mbar_init(&drained, 1);
     fence_mbar_init();
@@ -465,28 +505,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
   if (warp == 0 && elect_one()) {
-    const uint32_t bytes = 2 * (L::A_BYTES + (uint32_t)bn / 2 * KST);   // both CTAs' copies of a stage
+    const uint32_t bytes = 2 * stage_bytes;               // both CTAs' copies
     // Weights (and CTA 0's count of both CTAs' bytes of a stage). Weights that are
     // complete already need not wait for the kernel in front.
     if (!prefetch) pdl_wait();
-    const uint32_t base = smem_u32(ring) + L::A_BYTES, bars = mapa(smem_u32(full), 0);
+    const uint32_t base = smem_u32(ring) + spans * a_span, bars = mapa(smem_u32(full), 0);
     int s = 0;
     uint32_t ph = 1;
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
       const int nt = tile / tiles_m * cols;
       const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + bn / 2;
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = 0; c < stages; ++c) {
         if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
         if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-        tma_2d_pair(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
-        if (++s == L::NS) s = 0, ph ^= 1;
+        for (int g = 0; g < spans; ++g)
+          tma_2d_pair(base + s * stage_bytes + g * b_span, &tw, c * kst + g * (int)KST, n0, bars + 8 * s);
+        if (++s == ns) s = 0, ph ^= 1;
       }
     }
     // Copies still in flight after a wait that ran out count on CTA 0's barriers;
     // the cluster barrier below holds CTA 1 until CTA 0 has waited for them.
     if (!ok && rank == 0) {
       const uint64_t grace = globaltimer_ns() + timeout;
-      for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, grace);
+      for (int i = 0; i < ns; ++i) wait_phase(&full[i], 0, grace);
     }
   } else if (warp == 2 + PAIR_EPI && elect_one()) {
     pdl_wait();
@@ -494,13 +535,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     int s = 0;
     uint32_t ph = 1;
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
-      const int m0 = tile % tiles_m * 256 * MT + (int)rank * 128;
-      for (int c = 0; c < chunks; ++c) {
+      const int m0 = (tile % tiles_m * 2 + (int)rank) * tb;
+      for (int c = 0; c < stages; ++c) {
         if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          tma_2d_pair(base + s * L::STAGE + t * 128 * KST, &ta, c * (int)KST, m0 + 256 * t, bars + 8 * s);
-        if (++s == L::NS) s = 0, ph ^= 1;
+        for (int g = 0; g < spans; ++g)
+          tma_2d_pair(base + s * stage_bytes + g * a_span, &ta, c * kst + g * (int)KST, m0, bars + 8 * s);
+        if (++s == ns) s = 0, ph ^= 1;
       }
     }
   } else if (warp == 1 && rank == 0 && elect_one()) {
@@ -508,38 +548,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     int s = 0, it = 0;
     uint32_t ph = 0;
     for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
-      for (int c = 0; ok && c < chunks; ++c) {
-        uint64_t da = 0, db = 0;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const int b = MT == 1 ? it & 1 : t;             // accumulator
-          if (c == 0) ok = ok && wait_phase(&acc_empty[b], ((MT == 1 ? it >> 1 : it) & 1) ^ 1, deadline);
-          if (t == 0) {
-            ok = ok && wait_phase(&full[s], ph, deadline);
-            da = sdesc128(smem_u32(ring + (size_t)s * L::STAGE));
-            db = da + (L::A_BYTES >> 4);
-          }
-          if (!ok) break;
-          tc::fence_after_sync();
+      const int b = it & 1;
+      if (!(ok = wait_phase(&acc_empty[b], ((it >> 1) & 1) ^ 1, deadline))) break;
+      tc::fence_after_sync();
+      for (int c = 0; c < stages; ++c) {
+        if (!(ok = wait_phase(&full[s], ph, deadline))) break;
+        tc::fence_after_sync();
+        const uint64_t da = sdesc128(smem_u32(ring) + s * stage_bytes), db = da + (spans * a_span >> 4);
+        for (int g = 0; g < spans; ++g) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            mma_i8<2>(tmem + (uint32_t)(b * 256), da + t * (128 * KST >> 4) + 2 * j, db + 2 * j, idesc, c > 0 || j > 0);
-          if (MT == 2 && t == 0 && c == chunks - 1) commit_pair(&acc_full[0]);
+            mma_i8<2>(tmem + (uint32_t)(b * 256), da + g * (a_span >> 4) + 2 * j, db + g * (b_span >> 4) + 2 * j, idesc,
+                      c > 0 || g > 0 || j > 0);
         }
         commit_pair(&empty[s]);
-        if (++s == L::NS) s = 0, ph ^= 1;
+        if (++s == ns) s = 0, ph ^= 1;
       }
-      commit_pair(&acc_full[MT == 1 ? it & 1 : 1]);
+      commit_pair(&acc_full[b]);
     }
     commit_pair(&drained);
     wait_phase(&drained, 0, deadline + timeout);          // no MMA is in flight when TMEM is released
   } else if (warp >= 2 && warp < 2 + PAIR_EPI) {
     const int q = warp & 3, et = threadIdx.x - 64, h = warp >= 6;   // lane quarter, thread, warp group
-    uint8_t* stage = ring + L::NS * L::STAGE + (warp - 2) * 2 * PAIR_BLOCK;
+    uint8_t* stage = ring + PAIR_RING + (warp - 2) * 2 * PAIR_BLOCK;
     int buf = 0;
-    // One block per tile: the two warp groups take alternate pieces of 32 columns;
-    // two blocks: one each.
-    const int block = MT == 1 ? 0 : h, c_lo = MT == 1 ? 32 * h : 0, c_step = MT == 1 ? 64 : 32;
     pdl_wait();                                           // the tokens' scales, and the output's place
     // The scales one tile ahead: thread et's of a weight row, the lane's of a token.
     float next_w = 0.f, next_a = 0.f;
@@ -549,14 +581,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       if (tile >= tiles) return;
       const int tn = tile / tiles_m, n = tn * cols + (et < cols ? et : et - cols);
       next_n = tn * cols;
-      next_row = (int64_t)(tile - tn * tiles_m) * (256 * MT) + block * 256 + (int)rank * 128 + q * 32;
+      next_row = (int64_t)((tile - tn * tiles_m) * 2 + (int)rank) * tb + q * 32;
       next_w = et < bn && n < p.n ? __ldcg(&p.sw[et < cols ? n : p.n + n]) : 0.f;
       next_a = next_row + lane < p.m ? __ldcg(&p.sa[next_row + lane]) : 0.f;
     };
     look_ahead(pair);
     int it = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++it) {
-      const int b = MT == 1 ? it & 1 : h;                 // accumulator
+      const int b = it & 1;                               // accumulator
       const int n0 = next_n;
       const int64_t row0 = next_row;
       const float sa = next_a;
@@ -564,12 +596,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       sws[et] = next_w;
       look_ahead(tile + pairs);
       if (!epilogue_and(ok)) break;                       // this tile's sws are written; a wait that ran out ends all
-      ok = __all_sync(0xffffffffu, wait_phase(&acc_full[b], (MT == 1 ? it >> 1 : it) & 1, deadline));
+      ok = __all_sync(0xffffffffu, wait_phase(&acc_full[b], (it >> 1) & 1, deadline));
       if (!ok) continue;
       tc::fence_after_sync();
       const uint32_t t0 = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);
+      const int rows = (int)min((int64_t)(tb - q * 32), p.m - row0);       // this warp's tokens, of 32
 #pragma unroll 1
-      for (int c = c_lo; c < cols && n0 + c < p.n; c += c_step) {
+      for (int c = 32 * h; rows > 0 && c < cols && n0 + c < p.n; c += 64) {   // the groups' alternate pieces
         int32_t g[32];
         float v[32];
         tm_ld32(t0 + c, g);
@@ -588,13 +621,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
             v[j + 1] = swiglu(v[j + 1], r.y, p.limit, p.has_limit);
           }
         }
-        if (row0 >= p.m) continue;
         if (p.type != QX_T_F32) {
-          store_block<32>(p, &to, stage + buf * PAIR_BLOCK, row0, n0 + c, v, tma, lane);
+          store_block<32>(p, &to, stage + buf * PAIR_BLOCK, row0, rows, n0 + c, v, tma, lane);
           buf ^= 1;
         } else {
-          store_block<16>(p, &to, stage + buf * PAIR_BLOCK, row0, n0 + c, v, tma, lane);
-          if (n0 + c + 16 < p.n) store_block<16>(p, &to, stage + (buf ^ 1) * PAIR_BLOCK, row0, n0 + c + 16, v + 16, tma, lane);
+          store_block<16>(p, &to, stage + buf * PAIR_BLOCK, row0, rows, n0 + c, v, tma, lane);
+          if (n0 + c + 16 < p.n) store_block<16>(p, &to, stage + (buf ^ 1) * PAIR_BLOCK, row0, rows, n0 + c + 16, v + 16, tma, lane);
           else buf ^= 1;
         }
       }
@@ -606,7 +638,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   }
   __syncwarp();
   tc::fence_before_sync();
-  cluster_sync();
+  cluster_arrive_relaxed();
+  cluster_wait();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

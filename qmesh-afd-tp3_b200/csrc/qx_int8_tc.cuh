@@ -1,7 +1,7 @@
 // Tensor-core kernels of the int8 product (tcgen05.mma.kind::i8, int8 x int8
 // into int32 accumulators in TMEM), operands brought in by tiled TMA copies with
-// the 128-byte swizzle: a stage of the shared-memory ring is 256 bytes of K of the
-// operand tiles' rows, eight MMAs of K = 32.
+// the 128-byte swizzle: a stage of the shared-memory ring is one or two spans of 128
+// bytes of K of the operand tiles' rows, four MMAs of K = 32 each.
 //
 //   split_kernel  few tokens: weights are the M = 128 operand, tokens the N
 //                 operand, and the CTAs of a cluster split K (their sums, whole
@@ -18,10 +18,8 @@
 namespace qx {
 namespace i8 {
 
-// One swizzle span of K per tiled copy. A stage of a ring holds two of them (large
-// tiles of the pair kernel: one), so that the issuing threads' waits and loop, about
-// 300 cycles, are paid once per 256 bytes of K. K past the end reads as 0.
-constexpr uint32_t KST = 128, KSTAGE = 2 * KST;
+// K bytes of one tiled copy: a swizzle span. K past the end reads as 0.
+constexpr uint32_t KST = 128;
 
 // ---- descriptors -----------------------------------------------------------------
 // Shared-memory descriptor of a K-major tile with the 128-byte swizzle: rows 128
@@ -98,12 +96,8 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-__device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr));
-  return v;
+__device__ __forceinline__ void st_cluster(uint32_t addr, int32_t v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 // Arrive on another CTA's barrier. CTA scope: it says that accumulator reads are
 // done and publishes no memory; at cluster scope it would first wait for this
@@ -178,21 +172,22 @@ __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
 }
 
 // ------------------------------------------------------------------ few tokens
-// Grid: (row tile of 128 weight rows, token tile of BN tokens, K piece), the K
-// pieces of one tile in one cluster. Warps 0 and 6 copy weights and tokens (one
-// thread's copies for both took longer than their flight), warp 1 issues the MMAs,
-// warps 2-5 bring the accumulator to shared memory; then every CTA of the cluster adds
-// a share of the tile over the pieces and writes it. With SwiGLU the 128 rows are
-// 64 gate rows and their 64 up rows. The ring takes
-// half an SM, so that two CTAs run side by side.
+// Grid: (row tile of 128 weight rows) x (K piece), all tokens in one tile of BN, the K
+// pieces of a row tile in one cluster. Warps 0 and 6 copy weights and tokens (one
+// thread's copies for both took longer than their flight), warp 1 issues the MMAs.
+// Token t's sums meet in CTA t mod pieces: warps 2-5 of every CTA store theirs into
+// that CTA's shared memory, which adds them and writes the outputs. (Reading the
+// others' sums instead needs a second cluster barrier before a CTA may leave, 1.5 us.)
+// With SwiGLU the 128 rows are 64 gate rows and their 64 up rows. The weights' bytes
+// bound it, and at a few us the launch: 4608 x 5120 for one token streams 23.6 MB in
+// 3.8 of the kernel's 7 us. The ring takes half an SM, so that two CTAs run side by side.
 template <int BN>
 struct Split {
-  // a stage: two spans of 128 weight rows, then two of BN token rows
-  static constexpr uint32_t A_SPAN = 128 * KST, B_SPAN = BN * KST, A_BYTES = 2 * A_SPAN, STAGE = A_BYTES + 2 * B_SPAN;
+  static constexpr uint32_t A_BYTES = 128 * KST, STAGE = A_BYTES + BN * KST;
   static constexpr uint32_t COLS = BN < 32 ? 32 : BN;
-  static constexpr int NS = 114688 / STAGE;              // two CTAs per SM
-  static constexpr size_t SMEM = (size_t)NS * STAGE + 1024;   // 1024: alignment of the swizzled tiles
-  static_assert(BN * 128 * 4 <= NS * STAGE, "the accumulator fits the drained ring");
+  static constexpr uint32_t SUMS = (BN + 8) * 512;       // [piece][own token][128 rows], up to 8 pieces
+  static constexpr int NS = (114688 - SUMS) / STAGE;     // two CTAs per SM
+  static constexpr size_t SMEM = (size_t)NS * STAGE + SUMS + 1024;   // 1024: alignment of the swizzled tiles
 };
 constexpr int SPLIT_THR = 224;
 
@@ -205,13 +200,16 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   __shared__ uint64_t full[L::NS], empty[L::NS], done;
   __shared__ uint32_t tmem;
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
+  const uint32_t sums = smem_u32(ring) + L::NS * L::STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = pieces > 1 ? (int)cluster_rank() : 0;
+  const int rank = (int)cluster_rank();
   const int half = p.swiglu ? 64 : 128;                  // output columns of a tile
-  const int n0 = (int)(blockIdx.x / pieces) * half, m0 = blockIdx.y * BN;
-  const int chunks = (p.k + (int)KSTAGE - 1) / (int)KSTAGE;
-  const int c0 = (int)((int64_t)chunks * rank / pieces), c1 = (int)((int64_t)chunks * (rank + 1) / pieces);
+  const int n0 = (int)(blockIdx.x / pieces) * half;
+  const int chunks = (p.k + (int)KST - 1) / (int)KST;
+  const int c0 = chunks * rank / pieces, c1 = chunks * (rank + 1) / pieces;
+  const int own = (p.m + pieces - 1) / pieces;           // tokens per CTA at most
   pdl_launch_dependents();
+  cluster_arrive_relaxed();                              // this CTA's shared memory may be written
   if (threadIdx.x == 0) {
     prefetch_map(&tw);
     prefetch_map(&ta);
@@ -240,13 +238,8 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
       mbar_arrive_expect_tx(&full[s], L::STAGE);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = c * (int)KSTAGE + h * (int)KST;
-        const uint32_t to = base + s * L::STAGE + h * L::A_SPAN;
-        tma_2d(to, &tw, k, n0, bars + 8 * s);
-        if (p.swiglu) tma_2d(to + 64 * KST, &tw, k, p.n + n0, bars + 8 * s);
-      }
+      tma_2d(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
+      if (p.swiglu) tma_2d(base + s * L::STAGE + 64 * KST, &tw, c * (int)KST, p.n + n0, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
     if (!ok) {                                            // copies still in flight land before the CTA leaves
@@ -260,9 +253,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        tma_2d(base + s * L::STAGE + h * L::B_SPAN, &ta, c * (int)KSTAGE + h * (int)KST, m0, bars + 8 * s);
+      tma_2d(base + s * L::STAGE, &ta, c * (int)KST, 0, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
   } else if (warp == 1 && elect_one()) {
@@ -271,64 +262,58 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&full[s], ph, deadline))) break;
       tc::fence_after_sync();
-      const uint64_t da = sdesc128(smem_u32(ring + (size_t)s * L::STAGE)), db = da + (L::A_BYTES >> 4);
+      const uint64_t da = sdesc128(smem_u32(ring) + s * L::STAGE), db = da + (L::A_BYTES >> 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        mma_i8<1>(tmem, da + (j >> 2) * (L::A_SPAN >> 4) + 2 * (j & 3), db + (j >> 2) * (L::B_SPAN >> 4) + 2 * (j & 3),
-                  idesc_i8(128, BN), c > c0 || j > 0);
+      for (int j = 0; j < 4; ++j) mma_i8<1>(tmem, da + 2 * j, db + 2 * j, idesc_i8(128, BN), c > c0 || j > 0);
       tc::commit(&empty[s]);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
     tc::commit(&done);
   }
   __syncwarp();
-  const int cols = min(BN, p.m - m0);                     // tokens of the tile
-  int32_t* red = reinterpret_cast<int32_t*>(ring);        // [token][128 weight rows]
-  if (warp >= 2 && warp < 6) {
-    ok = wait_phase(&done, 0, deadline + timeout);
+  const bool epi = warp >= 2 && warp < 6;
+  if (epi) ok = wait_phase(&done, 0, deadline + timeout);
+  cluster_wait();                                         // every CTA of the cluster has started
+  if (epi && __all_sync(0xffffffffu, ok)) {
     tc::fence_after_sync();
-    if (__all_sync(0xffffffffu, ok)) {
-      const int q = warp & 3;
+    const int q = warp & 3;
+    uint32_t to = sums + (uint32_t)(rank * own * 128 + q * 32 + lane) * 4u;   // token t's place in its CTA
+    int dst = 0;                                          // t mod pieces
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 16) {
-        int32_t v[16];
-        tm_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+    for (int c = 0; c < p.m; c += 16) {
+      int32_t v[16];
+      tm_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c + i < cols) red[(c + i) * 128 + q * 32 + lane] = v[i];
+      for (int i = 0; i < 16; ++i) {
+        if (c + i < p.m) {
+          st_cluster(mapa(to, dst), v[i]);
+          if (++dst == pieces) dst = 0, to += 512;
+        }
       }
     }
     tc::fence_before_sync();
   }
   pdl_wait();                                             // the tokens' scales, and the output's place
-  if (pieces > 1) cluster_sync(); else __syncthreads();
-  // items: (token, four weight rows), dealt to the cluster's CTAs in even runs
-  const int per = half / 4, items = cols * per;
-  const int i0 = items * rank / pieces, i1 = items * (rank + 1) / pieces;
-  const uint32_t mine = smem_u32(red);
+  cluster_sync();
+  if (warp == 1) tc::tmem_dealloc(tmem, L::COLS);
+  // items of this CTA: (own token, four weight rows)
+  const int per = half / 4, items = (p.m - rank + pieces - 1) / pieces * per;
   const int four = p.type == QX_T_F32 ? 16 : 8;           // bytes of four outputs
   const bool vec = reinterpret_cast<uintptr_t>(p.out) % four == 0 && p.os % 4 == 0;
-  for (int i = i0 + (int)threadIdx.x; i < i1; i += SPLIT_THR) {
-    const int t = i / per, r = (i - t * per) * 4, n = n0 + r;
-    const uint32_t own = mine + (uint32_t)(t * 128 + r) * 4u;
-    int4 part[8], up[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {                          // every piece's sums requested at once
-      if (s < pieces) {
-        const uint32_t from = pieces > 1 ? mapa(own, s) : own;
-        part[s] = ld_cluster_int4(from);
-        if (p.swiglu) up[s] = ld_cluster_int4(from + 64 * 4);
+  const int32_t* sum = reinterpret_cast<const int32_t*>(ring + L::NS * L::STAGE);
+  for (int i = threadIdx.x; i < items; i += SPLIT_THR) {
+    const int tl = i / per, r = (i - tl * per) * 4, n = n0 + r, t = tl * pieces + rank;
+    int4 g = make_int4(0, 0, 0, 0), u = g;
+    for (int s = 0; s < pieces; ++s) {
+      const int32_t* from = sum + (s * own + tl) * 128 + r;
+      const int4 a = *reinterpret_cast<const int4*>(from);
+      g.x += a.x; g.y += a.y; g.z += a.z; g.w += a.w;
+      if (p.swiglu) {
+        const int4 b = *reinterpret_cast<const int4*>(from + 64);
+        u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
       }
     }
-    int4 g = part[0], u = up[0];
-#pragma unroll
-    for (int s = 1; s < 8; ++s) {
-      if (s < pieces) {
-        g.x += part[s].x; g.y += part[s].y; g.z += part[s].z; g.w += part[s].w;
-        if (p.swiglu) { u.x += up[s].x; u.y += up[s].y; u.z += up[s].z; u.w += up[s].w; }
-      }
-    }
-    const float sa = __ldcg(&p.sa[m0 + t]);
+    const float sa = __ldcg(&p.sa[t]);
     const int gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
     float v[4];
 #pragma unroll
@@ -337,7 +322,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       v[j] = scaled(gv[j], sa, __ldcg(&p.sw[nj]));
       if (p.swiglu) v[j] = swiglu(v[j], scaled(uv[j], sa, __ldcg(&p.sw[p.n + nj])), p.limit, p.has_limit);
     }
-    const int64_t at = (int64_t)(m0 + t) * p.os + n;
+    const int64_t at = (int64_t)t * p.os + n;
     if (vec && n + 4 <= p.n) {
       if (p.type == QX_T_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
       else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) =
@@ -348,13 +333,6 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
         if (n + j < p.n) store_out(p.out, at + j, p.type, v[j]);
     }
   }
-  // No CTA leaves before the others have read its sums.
-  __syncwarp();
-  if (pieces > 1) {
-    cluster_arrive_relaxed();
-    cluster_wait();
-  }
-  if (warp == 1) tc::tmem_dealloc(tmem, L::COLS);
 }
 
 // ------------------------------------------------------------------ many tokens

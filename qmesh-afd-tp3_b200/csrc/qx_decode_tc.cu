@@ -213,7 +213,7 @@ struct Params {
   int64_t xshared_stride;
   int xrank, xworld, xdst, xrows_max;
   // whole MoE layer (qx_moe_decode_tc): ids and tw are selected from the logits
-  float* logits;          // [rows][E], written by moe_front_kernel
+  float* logits;          // [rows][E rounded up to 4], written by moe_front_kernel
   const void* gate;       // router weights [E][HID], BF16 or FP32, rows gate_stride elements apart
   int64_t gate_stride;
   const float* gate_bias; // [E] or null
@@ -222,6 +222,7 @@ struct Params {
   const float* addend;    // optional FP32 [rows][HID] added before the output's rounding
   int64_t addend_stride;
   int sel_off;            // shared-memory offset of the selected ids [P], then weights [P]
+  int sel_warps;          // warps that select: their keys fit the ring
 };
 
 struct ItemMeta {
@@ -1492,7 +1493,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     // The logits are the front kernel's: wait for it, then select every row's
     // experts (each CTA all rows, a warp per row; CTA 0 also writes them out).
     pdl_wait();
-    select_rows(p, sel, reinterpret_cast<float*>(sel + p.P), warp, NTHR / 32);
+    select_rows(p, reinterpret_cast<uint32_t*>(ring), sel, reinterpret_cast<float*>(sel + p.P), warp, p.sel_warps);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after the keys
     __syncthreads();
     if (warp == 0) load_ids(p, sel, threadIdx.x & 31, idr);
   }
@@ -1608,7 +1610,7 @@ size_t qx_slice_workspace_tc_bytes(int32_t rows, int32_t topk, int32_t c0, int32
 size_t qx_moe_workspace_bytes(int32_t rows, int32_t n_experts, int32_t topk, int32_t c0, int32_t c1) {
   const size_t n = qx_slice_workspace_tc_bytes(rows, topk, c0, c1);
   if (n == 0 || n_experts < 1 || n_experts > MAXE || topk > n_experts) return 0;
-  return n + (size_t)rows * n_experts * sizeof(float);   // the slice's, then the logits
+  return n + (size_t)rows * ((n_experts + 3) & ~3) * sizeof(float);   // the slice's, then the logits
 }
 
 }  // extern "C"
@@ -1709,6 +1711,8 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   p.ring_bytes = (int)(SMEM_LIMIT - (size_t)p.ring_off);
   if (p.ring_bytes - 512 < 2 * (A_STAGE + p.bst)) return QX_ERR_SHAPE;   // two slots of the widest group
   p.ns = p.b_off = 0;
+  p.sel_warps = p.ring_bytes / (((arena->n_experts + 3) & ~3) * 4);
+  if (p.sel_warps > NTHR / 32) p.sel_warps = NTHR / 32;
   p.timeout_ns = timeout_ns();
   p.dep_extra = dep_extra();
   // With the clamp, |act| = |silu(min(g, L)) * clamp(u, -L, L)| <= L^2: one

@@ -213,7 +213,7 @@ struct Params {
   int64_t xshared_stride;
   int xrank, xworld, xdst, xrows_max;
   // whole MoE layer (qx_moe_decode_tc): ids and tw are selected from the logits
-  float* logits;          // [rows][E rounded up to 4], written by moe_front_kernel
+  float* logits;          // [quarter of K][rows][E rounded up to 4], written by moe_front_kernel
   const void* gate;       // router weights [E][HID], BF16 or FP32, rows gate_stride elements apart
   int64_t gate_stride;
   const float* gate_bias; // [E] or null
@@ -381,15 +381,12 @@ constexpr int IDR = MAXP / 32;   // expert ids per lane of the routing warp
 
 // Lane `lane`'s expert ids (pairs lane + 32 i); ids outside [0, E) (the -1
 // sentinel, or bad ids that the prep kernel flags) become -1 and are skipped.
-// `sel`: the ids selected in this CTA's shared memory (a whole MoE layer), or null.
-__device__ __forceinline__ void load_ids(const Params& p, const int32_t* sel, int lane, int (&idr)[IDR]) {
+__device__ __forceinline__ void load_ids(const Params& p, int lane, int (&idr)[IDR]) {
 #pragma unroll
   for (int i = 0; i < IDR; ++i) {
     const int q = lane + 32 * i;
     long long id = -1;
-    if (q < p.P && sel)
-      id = sel[q];
-    else if (q < p.P)
+    if (q < p.P)
       id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + q)
                    : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + q);
     idr[i] = (id >= 0 && id < p.E) ? (int)id : -1;
@@ -432,8 +429,10 @@ __device__ __forceinline__ int div_small(int a, int b) {
   return q;
 }
 
+// `sorted`: the call's keys in order (rank_keys), or null (the warp sorts them itself).
 template <int K>
-__device__ void route_sort(const Params& p, const int (&idr)[IDR], GroupS* gs, PairS* ps, RouteHdr* hdr) {
+__device__ void route_sort(const Params& p, const int (&idr)[IDR], const uint32_t* sorted, GroupS* gs, PairS* ps,
+                           RouteHdr* hdr) {
   static_assert(K <= IDR && (K & (K - 1)) == 0, "keys per lane");
   constexpr uint32_t FULL = 0xffffffffu, NONE = 0xffffffffu;
   constexpr int N = 32 * K;
@@ -445,7 +444,10 @@ __device__ void route_sort(const Params& p, const int (&idr)[IDR], GroupS* gs, P
     const int q = lane + 32 * j;
     v[j] = (q < p.P && idr[j] >= 0) ? ((uint32_t)idr[j] << 9) | (uint32_t)q : NONE;
   }
-  if constexpr (K == 2) {
+  if (sorted) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) v[j] = K * lane + j < p.P ? sorted[K * lane + j] : NONE;
+  } else if constexpr (K == 2) {
     // Up to 64 keys: a rank sort. A key's place is the number of smaller keys
     // (the valid keys are distinct: the pair index is in their low bits; the
     // equal NONE keys sort after them and are not placed); one short loop of
@@ -649,11 +651,12 @@ __device__ void route_finish(const Params& p, GroupS* gs, PairS* ps, RouteHdr* h
   __syncwarp();
 }
 
-__device__ void route_local(const Params& p, const int (&idr)[IDR], GroupS* gs, PairS* ps, RouteHdr* hdr) {
-  if (p.P <= 64) route_sort<2>(p, idr, gs, ps, hdr);
-  else if (p.P <= 128) route_sort<4>(p, idr, gs, ps, hdr);
-  else if (p.P <= 256) route_sort<8>(p, idr, gs, ps, hdr);
-  else route_sort<16>(p, idr, gs, ps, hdr);
+__device__ __forceinline__ void route_local(const Params& p, const int (&idr)[IDR], const uint32_t* sorted, GroupS* gs,
+                                            PairS* ps, RouteHdr* hdr) {
+  if (p.P <= 64) route_sort<2>(p, idr, sorted, gs, ps, hdr);
+  else if (p.P <= 128) route_sort<4>(p, idr, sorted, gs, ps, hdr);
+  else if (p.P <= 256) route_sort<8>(p, idr, sorted, gs, ps, hdr);
+  else route_sort<16>(p, idr, sorted, gs, ps, hdr);
   route_finish(p, gs, ps, hdr);
 }
 
@@ -662,11 +665,11 @@ __device__ void route_local(const Params& p, const int (&idr)[IDR], GroupS* gs, 
 // row computes the same), and the chunk's 16 unscaled x terms
 // q_t = rne(r_t / 2^(E - 2t)) (two elements per thread) into the row's stage
 // block. CTA 0 also resets the call's counters and records bad ids.
-// `units`: CTAs that run it; `given`: the call's ids are an input (to be checked).
-__device__ __forceinline__ void prep_unit(const Params& p, int units, bool given) {
+// `unit` of `units` CTAs; `given`: the call's ids are an input (to be checked).
+__device__ __forceinline__ void prep_unit(const Params& p, int unit, int units, bool given) {
   __shared__ float red[PREP_THR / 32];
   const int tid = threadIdx.x, lane = tid & 31;
-  if (blockIdx.x == 0) {
+  if (unit == 0) {
     bool bad = false;
     for (int q = tid; q < p.P + p.rows; q += PREP_THR) {
       if (given && q < p.P) {
@@ -685,9 +688,9 @@ __device__ __forceinline__ void prep_unit(const Params& p, int units, bool given
     __syncthreads();
     if (tid == 0 && bad) p.ctl->status = (uint32_t)QX_DEV_BAD_ID;
   }
-  for (int i = blockIdx.x * PREP_THR + tid; i < MAXSPLIT + MAXSG * MAX_STILES; i += units * PREP_THR)
+  for (int i = unit * PREP_THR + tid; i < MAXSPLIT + MAXSG * MAX_STILES; i += units * PREP_THR)
     p.pcnt[i] = 0;
-  const int r = blockIdx.x / NXCH, c = blockIdx.x - r * NXCH;
+  const int r = unit / NXCH, c = unit - r * NXCH;
   float inv = 1.f;
   if (p.x_fmt == QX_X_E4M3) inv = p.x_scale[r];
   else if (p.x_fmt == QX_X_E4M3_POST) inv = p.x_scale[0];
@@ -711,7 +714,7 @@ __device__ __forceinline__ void prep_unit(const Params& p, int units, bool given
 
 __global__ void __launch_bounds__(PREP_THR) tc_prep_kernel(Params p) {
   pdl_launch_dependents();
-  prep_unit(p, gridDim.x, true);
+  prep_unit(p, blockIdx.x, gridDim.x, true);
 }
 
 #include "qx_router.cuh"
@@ -1449,7 +1452,8 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   // Warp 0 loads the call's expert ids while other warps set up the CTA.
   int idr[IDR];
   int32_t* sel = MOE ? reinterpret_cast<int32_t*>(smem + p.sel_off) : nullptr;
-  if (!MOE && warp == 0) load_ids(p, nullptr, threadIdx.x & 31, idr);
+  uint32_t* sorted = nullptr;
+  if (!MOE && warp == 0) load_ids(p, threadIdx.x & 31, idr);
   if (threadIdx.x == 64) {
     for (int s = 0; s < MAXNS; ++s) {
       mbar_init(&S.full[s], 1);
@@ -1494,14 +1498,16 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     // experts (each CTA all rows, a warp per row; CTA 0 also writes them out).
     pdl_wait();
     select_rows(p, reinterpret_cast<uint32_t*>(ring), sel, reinterpret_cast<float*>(sel + p.P), warp, p.sel_warps);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after the keys
     __syncthreads();
-    if (warp == 0) load_ids(p, sel, threadIdx.x & 31, idr);
+    sorted = reinterpret_cast<uint32_t*>(ring);
+    rank_keys(p, sel, sorted, sorted + MAXP);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after these
+    __syncthreads();
   }
   // Otherwise the ids come from work before the prep kernel (which is launched without
   // early start), so the routing needs no wait; the prep kernel's results are
   // waited for by the threads that read them (producer, epilogue).
-  if (warp == 0) route_local(p, idr, gs, ps, &S.hdr);
+  if (warp == 0) route_local(p, idr, sorted, gs, ps, &S.hdr);
   pdl_launch_dependents();
   __syncwarp();
   tc::fence_before_sync();
@@ -1610,7 +1616,7 @@ size_t qx_slice_workspace_tc_bytes(int32_t rows, int32_t topk, int32_t c0, int32
 size_t qx_moe_workspace_bytes(int32_t rows, int32_t n_experts, int32_t topk, int32_t c0, int32_t c1) {
   const size_t n = qx_slice_workspace_tc_bytes(rows, topk, c0, c1);
   if (n == 0 || n_experts < 1 || n_experts > MAXE || topk > n_experts) return 0;
-  return n + (size_t)rows * ((n_experts + 3) & ~3) * sizeof(float);   // the slice's, then the logits
+  return n + (size_t)RSPLIT * rows * ((n_experts + 3) & ~3) * sizeof(float);   // the slice's, then the logits
 }
 
 }  // extern "C"

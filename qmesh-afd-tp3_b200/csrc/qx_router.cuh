@@ -3,17 +3,21 @@
 // the experts in every CTA of the decode kernel.
 
 // ------------------------------------------------------------------ logits
-// One CTA: 16 rows x 8 experts over all of K, on warp-level BF16 tensor-core products
-// (m16n8k16; the 16 x 8 tile is too small for a TMEM accumulator to pay). Warp w takes
-// an eighth of K in 20 blocks of 32; a lane reads 8 consecutive elements of its row
-// and of its expert, which are the operands of two products under one and the same
-// permutation of K. Products of BF16 values are exact; FP32 router weights enter as
-// three BF16 parts, w = hi + mid + lo to 2^-26. Each block's sum starts from zero and
-// is added in FP32, so that a logit's error stays near 2^-24 of its partial sums.
-// Bound by latency: the tile's weights and rows are asked into L2 at once, so that the
-// blocks' loads wait for L2 only (13 -> 7 us with one row).
-constexpr int RE = 8, RR = 16, RWARPS = PREP_THR / 32, RK = HID / RWARPS;
+// One CTA: 16 rows x 8 experts over a quarter of K, on warp-level BF16 tensor-core
+// products (m16n8k16; the 16 x 8 tile is too small for a TMEM accumulator to pay).
+// Each of its 8 warps takes 160 elements in 5 blocks of 32, every load of which is in
+// flight at once: the weights' way from memory, paid once, is all that bounds it (one
+// CTA over all of K, four rounds of loads, took 9 us with one row). A lane reads 8
+// consecutive elements of its row and of its expert, which are the operands of two
+// products under one and the same permutation of K. Products of BF16 values are exact;
+// FP32 router weights enter as three BF16 parts, w = hi + mid + lo to 2^-26. Each
+// block's sum starts from zero and is added in FP32, so that a logit's error stays near
+// 2^-24 of its partial sums; the quarters' sums are added where the logits are read.
+constexpr int RE = 8, RR = 16, RWARPS = PREP_THR / 32, RSPLIT = 4, RK = HID / RSPLIT / RWARPS, RB = RK / 32;
 static_assert(RK % 32 == 0, "whole blocks of K per warp");
+
+// Floats between the quarters' logits, [rows][E rounded up to 4] each.
+__device__ __forceinline__ int logit_row(const Params& p) { return (p.E + 3) & ~3; }
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -35,11 +39,6 @@ __device__ __forceinline__ uint4 load_x8(const Params& p, const uint8_t* xr, int
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// A run of memory towards L2 (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void prefetch_l2(const uint8_t* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
 // c += a b over 16 elements of K (the k-th pairs of both operands belong together).
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
@@ -50,54 +49,62 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 }
 
 template <int GT>
-__device__ __forceinline__ void router_unit(const Params& p, int e0, int r0) {
+__device__ __forceinline__ void router_unit(const Params& p, int e0, int r0, int quarter) {
   __shared__ __align__(8) float part[RWARPS][RR][RE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool two = r0 + 8 < p.rows;                      // the tile has rows 8..15
   const int ra = min(r0 + g, p.rows - 1), rb = min(r0 + g + 8, p.rows - 1);
   const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x);
-  const uint8_t *xa = x + (size_t)ra * p.x_stride, *xb = x + (size_t)rb * p.x_stride;
   float ia = 1.f, ib = 1.f;
   if (p.x_fmt == QX_X_E4M3) ia = p.x_scale[ra], ib = p.x_scale[rb];
   else if (p.x_fmt == QX_X_E4M3_POST) ia = ib = p.x_scale[0];
-  const size_t at = (size_t)min(e0 + g, p.E - 1) * p.gate_stride;
-  constexpr int GB = GT == QX_T_BF16 ? 2 : 4;
-  if ((int)threadIdx.x < RE) {
-    if (e0 + (int)threadIdx.x < p.E)
-      prefetch_l2(reinterpret_cast<const uint8_t*>(p.gate) + (size_t)(e0 + threadIdx.x) * p.gate_stride * GB, HID * GB);
-  } else if ((int)threadIdx.x < RE + RR && r0 + (int)threadIdx.x - RE < p.rows) {
-    prefetch_l2(x + (size_t)(r0 + threadIdx.x - RE) * p.x_stride, p.x_fmt == QX_X_BF16 ? 2 * HID : HID);
+  const int k0 = (quarter * RWARPS + warp) * RK + 8 * t;
+  const size_t at = (size_t)min(e0 + g, p.E - 1) * p.gate_stride + k0;
+  constexpr int GV = GT == QX_T_BF16 ? 1 : 2;            // 16-byte pieces of 8 weights
+  uint4 va[RB], vb[RB], wv[RB][GV];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const uint8_t* gp = reinterpret_cast<const uint8_t*>(p.gate) + (at + 32 * i) * (8 * GV / 4);
+#pragma unroll
+    for (int v = 0; v < GV; ++v) wv[i][v] = *reinterpret_cast<const uint4*>(gp + 16 * v);
+  }
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    va[i] = load_x8(p, x + (size_t)ra * p.x_stride, k0 + 32 * i, ia);
+    vb[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (two) vb[i] = load_x8(p, x + (size_t)rb * p.x_stride, k0 + 32 * i, ib);
   }
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll (GT == QX_T_BF16 ? 10 : 5)
-  for (int k = warp * RK + 8 * t; k < (warp + 1) * RK; k += 32) {
-    const uint4 va = load_x8(p, xa, k, ia), vb = two ? load_x8(p, xb, k, ib) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const uint4 a = va[i], b = vb[i];
     float c[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (GT == QX_T_BF16) {
-      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.gate) + at + k);
-      mma16(c, va.x, vb.x, va.y, vb.y, w.x, w.y);
-      mma16(c, va.z, vb.z, va.w, vb.w, w.z, w.w);
+      const uint4 w = wv[i][0];
+      mma16(c, a.x, b.x, a.y, b.y, w.x, w.y);
+      mma16(c, a.z, b.z, a.w, b.w, w.z, w.w);
     } else {
-      const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + at + k);
-      const float4 f0 = f[0], f1 = f[1];
-      float v[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+      const uint32_t f[8] = {wv[i][0].x, wv[i][0].y, wv[i][0].z, wv[i][0].w,
+                             wv[i][GV - 1].x, wv[i][GV - 1].y, wv[i][GV - 1].z, wv[i][GV - 1].w};
       uint32_t w[3][4];
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int j = 0; j < 4; ++j) {
+        float lo = __uint_as_float(f[2 * j]), hi = __uint_as_float(f[2 * j + 1]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[q][i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-          v[2 * i] -= bf16_lo(w[q][i]);
-          v[2 * i + 1] -= bf16_hi(w[q][i]);
+        for (int q = 0; q < 3; ++q) {
+          w[q][j] = bf16_pair(lo, hi);
+          lo -= bf16_lo(w[q][j]);
+          hi -= bf16_hi(w[q][j]);
         }
+      }
 #pragma unroll
       for (int q = 2; q >= 0; --q) {                      // the small parts first
-        mma16(c, va.x, vb.x, va.y, vb.y, w[q][0], w[q][1]);
-        mma16(c, va.z, vb.z, va.w, vb.w, w[q][2], w[q][3]);
+        mma16(c, a.x, b.x, a.y, b.y, w[q][0], w[q][1]);
+        mma16(c, a.z, b.z, a.w, b.w, w[q][2], w[q][3]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += c[i];
+    for (int j = 0; j < 4; ++j) acc[j] += c[j];
   }
   *reinterpret_cast<float2*>(&part[warp][g][2 * t]) = make_float2(acc[0], acc[1]);
   *reinterpret_cast<float2*>(&part[warp][g + 8][2 * t]) = make_float2(acc[2], acc[3]);
@@ -107,25 +114,26 @@ __device__ __forceinline__ void router_unit(const Params& p, int e0, int r0) {
     float s = part[0][r][e];
 #pragma unroll
     for (int w = 1; w < RWARPS; ++w) s += part[w][r][e];
-    p.logits[(size_t)(r0 + r) * ((p.E + 3) & ~3) + e0 + e] = p.gate_bias ? s + __ldg(&p.gate_bias[e0 + e]) : s;
+    if (quarter == 0 && p.gate_bias) s += __ldg(&p.gate_bias[e0 + e]);
+    p.logits[((size_t)quarter * p.rows + r0 + r) * logit_row(p) + e0 + e] = s;
   }
 }
 
-// CTAs [0, rows * NXCH): the x terms; then one per (8 experts, 16 rows).
+// CTAs: one per (8 experts, 16 rows, quarter of K), then the x terms' rows * NXCH.
 template <int GT>
 __global__ void __launch_bounds__(PREP_THR) moe_front_kernel(Params p) {
   pdl_launch_dependents();
-  const int prep = p.rows * NXCH;
-  if ((int)blockIdx.x < prep) {
-    prep_unit(p, prep, false);
+  const int prep = p.rows * NXCH, first = (int)gridDim.x - prep;
+  if ((int)blockIdx.x >= first) {
+    prep_unit(p, (int)blockIdx.x - first, prep, false);
     return;
   }
-  const int u = blockIdx.x - prep, ne = (p.E + RE - 1) / RE;
-  router_unit<GT>(p, u % ne * RE, u / ne * RR);
+  const int ne = (p.E + RE - 1) / RE, u = blockIdx.x, tile = u / RSPLIT;
+  router_unit<GT>(p, tile % ne * RE, tile / ne * RR, u % RSPLIT);
 }
 
 static void front_launch(const Params& p, int gate_type, cudaStream_t st) {
-  const int grid = p.rows * NXCH + (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR);
+  const int grid = p.rows * NXCH + (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR) * RSPLIT;
   if (gate_type == QX_T_BF16) moe_front_kernel<QX_T_BF16><<<grid, PREP_THR, 0, st>>>(p);
   else moe_front_kernel<QX_T_F32><<<grid, PREP_THR, 0, st>>>(p);
 }
@@ -146,13 +154,20 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 // words) while each lane keeps the best of its own; a round takes the largest over
 // the lanes (the lowest id of equals) and the lane it came from looks for its next.
 // Short loops rather than unrolled ones: every SM fetches this code cold, once per
-// call. Slot j's id and weight go to ids[j], tw[j].
-__device__ void select_row(const float* l, int E, int topk, int lane, uint32_t* keys, int32_t* ids, float* tw) {
+// call. `l`: the row's logits of the first quarter of K, the others' `step` floats
+// apart. Slot j's id and weight go to ids[j], tw[j].
+__device__ void select_row(const float* l, size_t step, int E, int topk, int lane, uint32_t* keys, int32_t* ids,
+                           float* tw) {
   uint32_t bk = 0u;                                       // 0: no key (every logit's is above it)
   int be = INT_MAX;
-#pragma unroll 4
+#pragma unroll 3
   for (int e = 4 * lane; e < E; e += 128) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(l + e));
+    float4 v = __ldcg(reinterpret_cast<const float4*>(l + e));
+#pragma unroll
+    for (int q = 1; q < RSPLIT; ++q) {
+      const float4 w = __ldcg(reinterpret_cast<const float4*>(l + q * step + e));
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
     const uint4 k = make_uint4(logit_key(v.x), e + 1 < E ? logit_key(v.y) : 0u, e + 2 < E ? logit_key(v.z) : 0u,
                                e + 3 < E ? logit_key(v.w) : 0u);
     *reinterpret_cast<uint4*>(keys + e) = k;
@@ -197,16 +212,40 @@ __device__ void select_row(const float* l, int E, int topk, int lane, uint32_t* 
 // Every row of the call into shared memory (ids[P], tw[P]), a warp per row; `keys`:
 // E4 words per warp.
 __device__ void select_rows(const Params& p, uint32_t* keys, int32_t* ids, float* tw, int warp, int warps) {
-  const int lane = threadIdx.x & 31, E4 = (p.E + 3) & ~3;
+  const int lane = threadIdx.x & 31, E4 = logit_row(p);
   if (warp >= warps) return;
 #pragma unroll 1
   for (int r = warp; r < p.rows; r += warps) {
     int32_t* ir = ids + r * p.topk;
     float* wr = tw + r * p.topk;
-    select_row(p.logits + (size_t)r * E4, p.E, p.topk, lane, keys + warp * E4, ir, wr);
+    select_row(p.logits + (size_t)r * E4, (size_t)p.rows * E4, p.E, p.topk, lane, keys + warp * E4, ir, wr);
     if (blockIdx.x == 0 && lane < p.topk) {
       if (p.ids_out) p.ids_out[r * p.topk + lane] = ir[lane];
       if (p.tw_out) p.tw_out[r * p.topk + lane] = wr[lane];
     }
+  }
+}
+
+// The call's keys (expert << 9 | pair; no expert: all ones) in ascending order, by all
+// threads of the CTA: a key's place is the number of smaller ones (the valid ones are
+// distinct), those without an expert follow. `sorted`, `keys`: MAXP words each. (A
+// sorting network in one warp took 24 us for 288 pairs.)
+__device__ void rank_keys(const Params& p, const int32_t* ids, uint32_t* sorted, uint32_t* keys) {
+  const int P4 = (p.P + 3) & ~3;
+  for (int i = threadIdx.x; i < P4; i += NTHR) {
+    const uint32_t k = i < p.P && ids[i] >= 0 ? (uint32_t)ids[i] << 9 | (uint32_t)i : 0xffffffffu;
+    keys[i] = k;
+    sorted[i] = 0xffffffffu;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.P; i += NTHR) {
+    const uint32_t k = keys[i];
+    int place = 0;
+#pragma unroll 2
+    for (int j = 0; j < P4; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(keys + j);
+      place += (int)(o.x < k) + (int)(o.y < k) + (int)(o.z < k) + (int)(o.w < k);
+    }
+    if (k != 0xffffffffu) sorted[place] = k;
   }
 }

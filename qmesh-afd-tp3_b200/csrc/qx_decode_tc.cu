@@ -57,10 +57,10 @@
 //                      tile's counter is complete, or hands them to the fused rank
 //                      combine (qx_xchg.cuh).
 //
-// A whole MoE layer (qx_moe_decode_tc) is the same pair with the router in
-// front: moe_front_kernel computes the router's logits beside the x terms, and
-// every CTA of tc_decode_kernel<true> selects the top-k from them itself before
-// it builds the routing tables, so the layer is two kernels.
+// A whole MoE layer (qx_moe_decode_tc) is the same with the router in front:
+// moe_router_kernel computes the logits while moe_prep_kernel computes the x terms,
+// and every CTA of tc_decode_kernel<true> selects the top-k from the logits itself
+// before it builds the routing tables.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
@@ -213,7 +213,7 @@ struct Params {
   int64_t xshared_stride;
   int xrank, xworld, xdst, xrows_max;
   // whole MoE layer (qx_moe_decode_tc): ids and tw are selected from the logits
-  float* logits;          // [quarter of K][rows][E rounded up to 4], written by moe_front_kernel
+  float* logits;          // [quarter of K][rows][E rounded up to 4], written by moe_router_kernel
   const void* gate;       // router weights [E][HID], BF16 or FP32, rows gate_stride elements apart
   int64_t gate_stride;
   const float* gate_bias; // [E] or null
@@ -429,10 +429,8 @@ __device__ __forceinline__ int div_small(int a, int b) {
   return q;
 }
 
-// `sorted`: the call's keys in order (rank_keys), or null (the warp sorts them itself).
 template <int K>
-__device__ void route_sort(const Params& p, const int (&idr)[IDR], const uint32_t* sorted, GroupS* gs, PairS* ps,
-                           RouteHdr* hdr) {
+__device__ void route_sort(const Params& p, const int (&idr)[IDR], GroupS* gs, PairS* ps, RouteHdr* hdr) {
   static_assert(K <= IDR && (K & (K - 1)) == 0, "keys per lane");
   constexpr uint32_t FULL = 0xffffffffu, NONE = 0xffffffffu;
   constexpr int N = 32 * K;
@@ -444,10 +442,7 @@ __device__ void route_sort(const Params& p, const int (&idr)[IDR], const uint32_
     const int q = lane + 32 * j;
     v[j] = (q < p.P && idr[j] >= 0) ? ((uint32_t)idr[j] << 9) | (uint32_t)q : NONE;
   }
-  if (sorted) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) v[j] = K * lane + j < p.P ? sorted[K * lane + j] : NONE;
-  } else if constexpr (K == 2) {
+  if constexpr (K == 2) {
     // Up to 64 keys: a rank sort. A key's place is the number of smaller keys
     // (the valid keys are distinct: the pair index is in their low bits; the
     // equal NONE keys sort after them and are not placed); one short loop of
@@ -651,12 +646,11 @@ __device__ void route_finish(const Params& p, GroupS* gs, PairS* ps, RouteHdr* h
   __syncwarp();
 }
 
-__device__ __forceinline__ void route_local(const Params& p, const int (&idr)[IDR], const uint32_t* sorted, GroupS* gs,
-                                            PairS* ps, RouteHdr* hdr) {
-  if (p.P <= 64) route_sort<2>(p, idr, sorted, gs, ps, hdr);
-  else if (p.P <= 128) route_sort<4>(p, idr, sorted, gs, ps, hdr);
-  else if (p.P <= 256) route_sort<8>(p, idr, sorted, gs, ps, hdr);
-  else route_sort<16>(p, idr, sorted, gs, ps, hdr);
+__device__ void route_local(const Params& p, const int (&idr)[IDR], GroupS* gs, PairS* ps, RouteHdr* hdr) {
+  if (p.P <= 64) route_sort<2>(p, idr, gs, ps, hdr);
+  else if (p.P <= 128) route_sort<4>(p, idr, gs, ps, hdr);
+  else if (p.P <= 256) route_sort<8>(p, idr, gs, ps, hdr);
+  else route_sort<16>(p, idr, gs, ps, hdr);
   route_finish(p, gs, ps, hdr);
 }
 
@@ -1452,7 +1446,6 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   // Warp 0 loads the call's expert ids while other warps set up the CTA.
   int idr[IDR];
   int32_t* sel = MOE ? reinterpret_cast<int32_t*>(smem + p.sel_off) : nullptr;
-  uint32_t* sorted = nullptr;
   if (!MOE && warp == 0) load_ids(p, threadIdx.x & 31, idr);
   if (threadIdx.x == 64) {
     for (int s = 0; s < MAXNS; ++s) {
@@ -1499,15 +1492,15 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     pdl_wait();
     select_rows(p, reinterpret_cast<uint32_t*>(ring), sel, reinterpret_cast<float*>(sel + p.P), warp, p.sel_warps);
     __syncthreads();
-    sorted = reinterpret_cast<uint32_t*>(ring);
-    rank_keys(p, sel, sorted, sorted + MAXP);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after these
+    route_pairs(p, sel, reinterpret_cast<uint32_t*>(ring), gs, ps, &S.hdr);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after this use of it
     __syncthreads();
+    if (warp == 0) route_finish(p, gs, ps, &S.hdr);
   }
   // Otherwise the ids come from work before the prep kernel (which is launched without
   // early start), so the routing needs no wait; the prep kernel's results are
   // waited for by the threads that read them (producer, epilogue).
-  if (warp == 0) route_local(p, idr, sorted, gs, ps, &S.hdr);
+  if (!MOE && warp == 0) route_local(p, idr, gs, ps, &S.hdr);
   pdl_launch_dependents();
   __syncwarp();
   tc::fence_before_sync();
@@ -1797,9 +1790,12 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   const size_t smem_bytes = SMEM_LIMIT;
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (rt) front_launch(p, rt->gate_type, st);
-  else tc_prep_kernel<<<a->rows * NXCH, PREP_THR, 0, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return QX_ERR_LAUNCH;
+  if (rt) {
+    if (front_launch(p, rt->gate_type, st) != cudaSuccess) return QX_ERR_LAUNCH;
+  } else {
+    tc_prep_kernel<<<a->rows * NXCH, PREP_THR, 0, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return QX_ERR_LAUNCH;
+  }
 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

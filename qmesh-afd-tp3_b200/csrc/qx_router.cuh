@@ -119,23 +119,40 @@ __device__ __forceinline__ void router_unit(const Params& p, int e0, int r0, int
   }
 }
 
-// CTAs: one per (8 experts, 16 rows, quarter of K), then the x terms' rows * NXCH.
+// CTAs: one per (8 experts, 16 rows, quarter of K).
 template <int GT>
-__global__ void __launch_bounds__(PREP_THR) moe_front_kernel(Params p) {
+__global__ void __launch_bounds__(PREP_THR) moe_router_kernel(Params p) {
   pdl_launch_dependents();
-  const int prep = p.rows * NXCH, first = (int)gridDim.x - prep;
-  if ((int)blockIdx.x >= first) {
-    prep_unit(p, (int)blockIdx.x - first, prep, false);
-    return;
-  }
   const int ne = (p.E + RE - 1) / RE, u = blockIdx.x, tile = u / RSPLIT;
   router_unit<GT>(p, tile % ne * RE, tile / ne * RR, u % RSPLIT);
 }
 
-static void front_launch(const Params& p, int gate_type, cudaStream_t st) {
-  const int grid = p.rows * NXCH + (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR) * RSPLIT;
-  if (gate_type == QX_T_BF16) moe_front_kernel<QX_T_BF16><<<grid, PREP_THR, 0, st>>>(p);
-  else moe_front_kernel<QX_T_F32><<<grid, PREP_THR, 0, st>>>(p);
+// The x terms beside the router: started with it (everything the call reads is
+// complete then) and ended after it, so that waiting for this kernel is waiting for
+// both. (One kernel for both ran the units at the router's registers: 13 us against
+// 7 with 48 rows.)
+__global__ void __launch_bounds__(PREP_THR) moe_prep_kernel(Params p) {
+  pdl_launch_dependents();
+  prep_unit(p, blockIdx.x, gridDim.x, false);
+  pdl_wait();
+}
+
+static cudaError_t front_launch(const Params& p, int gate_type, cudaStream_t st) {
+  const int grid = (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR) * RSPLIT;
+  if (gate_type == QX_T_BF16) moe_router_kernel<QX_T_BF16><<<grid, PREP_THR, 0, st>>>(p);
+  else moe_router_kernel<QX_T_F32><<<grid, PREP_THR, 0, st>>>(p);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.rows * NXCH, 1, 1);
+  cfg.blockDim = dim3(PREP_THR, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, moe_prep_kernel, p);
 }
 
 // ------------------------------------------------------------------ selection
@@ -150,16 +167,31 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k == 0xffffffffu ? 0x7fc00000u : k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// The topk experts of one row by one warp: the keys go to shared memory (`keys`, E4
-// words) while each lane keeps the best of its own; a round takes the largest over
-// the lanes (the lowest id of equals) and the lane it came from looks for its next.
-// Short loops rather than unrolled ones: every SM fetches this code cold, once per
-// call. `l`: the row's logits of the first quarter of K, the others' `step` floats
-// apart. Slot j's id and weight go to ids[j], tw[j].
+// The two largest (key, lowest id of equals) that a lane has seen, ids ascending.
+struct Top2 {
+  uint32_t k0 = 0u, k1 = 0u;                              // 0: none (every logit's key is above it)
+  int e0 = INT_MAX, e1 = INT_MAX;
+  __device__ __forceinline__ void add(uint32_t k, int e) {
+    if (k > k0) k1 = k0, e1 = e0, k0 = k, e0 = e;
+    else if (k > k1) k1 = k, e1 = e;
+  }
+  __device__ __forceinline__ void add4(const uint4& k, int e) {
+    add(k.x, e);
+    add(k.y, e + 1);
+    add(k.z, e + 2);
+    add(k.w, e + 3);
+  }
+};
+
+// The topk experts of one row by one warp: the keys go to shared memory (`keys`, one
+// row of logits) while each lane keeps its two best; a round takes the largest over
+// the lanes (the lowest id of equals), and a lane that has given both looks through
+// its keys again. Short loops rather than unrolled ones: every SM fetches this code
+// cold, once per call. `l`: the row's logits of the first quarter of K, the others'
+// `step` floats apart. Slot j's id and weight go to ids[j], tw[j].
 __device__ void select_row(const float* l, size_t step, int E, int topk, int lane, uint32_t* keys, int32_t* ids,
                            float* tw) {
-  uint32_t bk = 0u;                                       // 0: no key (every logit's is above it)
-  int be = INT_MAX;
+  Top2 best;
 #pragma unroll 3
   for (int e = 4 * lane; e < E; e += 128) {
     float4 v = __ldcg(reinterpret_cast<const float4*>(l + e));
@@ -171,29 +203,22 @@ __device__ void select_row(const float* l, size_t step, int E, int topk, int lan
     const uint4 k = make_uint4(logit_key(v.x), e + 1 < E ? logit_key(v.y) : 0u, e + 2 < E ? logit_key(v.z) : 0u,
                                e + 3 < E ? logit_key(v.w) : 0u);
     *reinterpret_cast<uint4*>(keys + e) = k;
-    if (k.x > bk) bk = k.x, be = e;
-    if (k.y > bk) bk = k.y, be = e + 1;
-    if (k.z > bk) bk = k.z, be = e + 2;
-    if (k.w > bk) bk = k.w, be = e + 3;
+    best.add4(k, e);
   }
   uint32_t my_key = 0u;
   int my_id = -1;
 #pragma unroll 1
   for (int j = 0; j < topk; ++j) {
-    const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
-    const int id = __reduce_min_sync(0xffffffffu, bk == best ? be : INT_MAX);
-    if (lane == j) my_key = best, my_id = best > KEY_NEG_INF ? id : -1;
-    if (be == id) {                                       // this lane's: out, and its next best
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best.k0);
+    const int id = __reduce_min_sync(0xffffffffu, best.k0 == top ? best.e0 : INT_MAX);
+    if (lane == j) my_key = top, my_id = top > KEY_NEG_INF ? id : -1;
+    if (best.e0 == id) {
       keys[id] = 0u;
-      bk = 0u;
-      be = INT_MAX;
+      best.k0 = best.k1, best.e0 = best.e1;
+      best.k1 = 0u, best.e1 = INT_MAX;
+      if (best.e0 == INT_MAX) {
 #pragma unroll 1
-      for (int e = 4 * lane; e < E; e += 128) {
-        const uint4 k = *reinterpret_cast<const uint4*>(keys + e);
-        if (k.x > bk) bk = k.x, be = e;
-        if (k.y > bk) bk = k.y, be = e + 1;
-        if (k.z > bk) bk = k.z, be = e + 2;
-        if (k.w > bk) bk = k.w, be = e + 3;
+        for (int e = 4 * lane; e < E; e += 128) best.add4(*reinterpret_cast<const uint4*>(keys + e), e);
       }
     }
     __syncwarp();
@@ -226,26 +251,77 @@ __device__ void select_rows(const Params& p, uint32_t* keys, int32_t* ids, float
   }
 }
 
-// The call's keys (expert << 9 | pair; no expert: all ones) in ascending order, by all
-// threads of the CTA: a key's place is the number of smaller ones (the valid ones are
-// distinct), those without an expert follow. `sorted`, `keys`: MAXP words each. (A
-// sorting network in one warp took 24 us for 288 pairs.)
-__device__ void rank_keys(const Params& p, const int32_t* ids, uint32_t* sorted, uint32_t* keys) {
-  const int P4 = (p.P + 3) & ~3;
-  for (int i = threadIdx.x; i < P4; i += NTHR) {
-    const uint32_t k = i < p.P && ids[i] >= 0 ? (uint32_t)ids[i] << 9 | (uint32_t)i : 0xffffffffu;
-    keys[i] = k;
-    sorted[i] = 0xffffffffu;
+// The routing tables of route_sort (unique experts ascending, an expert's pairs in
+// order, split evenly into groups of at most gmax) from the ids in shared memory, by
+// all threads of the CTA instead of one warp: a pair's place, its expert's first place
+// and pair count are counts over all pairs, a group's number a sum over the places
+// before its expert's. `scratch`: 2 MAXP words. (In one warp, sorting network and
+// scans took 41 us for 288 pairs.)
+__device__ void route_pairs(const Params& p, const int32_t* ids, uint32_t* scratch, GroupS* gs, PairS* ps,
+                            RouteHdr* hdr) {
+  constexpr uint32_t NONE = 0xffffffffu;
+  constexpr int PT = (MAXP + NTHR - 1) / NTHR;            // pairs per thread
+  const int P4 = (p.P + 3) & ~3, gmax = min(GMAX, p.rows), tid = threadIdx.x;
+  uint32_t *keys = scratch, *runs = scratch + MAXP;       // runs: at an expert's first place, its groups
+  for (int i = tid; i < P4; i += NTHR) {
+    keys[i] = i < p.P && ids[i] >= 0 ? (uint32_t)ids[i] << 9 | (uint32_t)i : NONE;
+    runs[i] = 0u;
   }
+  if (tid == 0) hdr->n_groups = hdr->n_pairs = hdr->b_max = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < p.P; i += NTHR) {
-    const uint32_t k = keys[i];
-    int place = 0;
+  int place[PT], start[PT], count[PT], valid = 0;
+#pragma unroll
+  for (int u = 0; u < PT; ++u) {
+    const int i = tid + u * NTHR;
+    place[u] = -1;
+    if (i >= p.P || keys[i] == NONE) continue;
+    const uint32_t k = keys[i], lo = k & ~511u, hi = k | 511u;   // the expert's keys lie in [lo, hi]
+    int below = 0, before = 0, upto = 0;
+    valid = 0;
 #pragma unroll 2
     for (int j = 0; j < P4; j += 4) {
       const uint4 o = *reinterpret_cast<const uint4*>(keys + j);
-      place += (int)(o.x < k) + (int)(o.y < k) + (int)(o.z < k) + (int)(o.w < k);
+      below += (int)(o.x < lo) + (int)(o.y < lo) + (int)(o.z < lo) + (int)(o.w < lo);
+      before += (int)(o.x < k) + (int)(o.y < k) + (int)(o.z < k) + (int)(o.w < k);
+      upto += (int)(o.x <= hi) + (int)(o.y <= hi) + (int)(o.z <= hi) + (int)(o.w <= hi);
+      valid += (int)(o.x != NONE) + (int)(o.y != NONE) + (int)(o.z != NONE) + (int)(o.w != NONE);
     }
-    if (k != 0xffffffffu) sorted[place] = k;
+    place[u] = before;
+    start[u] = below;
+    count[u] = upto - below;
+    ps[before].pq = i;
+    ps[before].row = div_small(i, p.topk);
+    if (before == below) runs[below] = (uint32_t)div_small(count[u] + gmax - 1, gmax);
+  }
+  __syncthreads();
+  const int abs = ((p.NT + SK - 1) / SK) * XT_STAGE;      // down-operand bytes per pair
+#pragma unroll
+  for (int u = 0; u < PT; ++u) {
+    if (place[u] < 0) continue;
+    const int c = count[u], r = place[u] - start[u], ng = div_small(c + gmax - 1, gmax);
+    const int gk = div_small((r + 1) * ng - 1, c);        // the k with k c / ng <= r < (k + 1) c / ng
+    const int lo = div_small(gk * c, ng);
+    if (r != lo) continue;                                // the group's first pair writes its record
+    int g = gk;
+    for (int j = 0; j < start[u]; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(runs + j);
+      g += (int)o.x + (j + 1 < start[u] ? (int)o.y : 0) + (j + 2 < start[u] ? (int)o.z : 0) +
+           (j + 3 < start[u] ? (int)o.w : 0);
+    }
+    GroupS d;
+    d.expert = (int)(keys[tid + u * NTHR] >> 9);
+    d.gsz = div_small((gk + 1) * c, ng) - lo;
+    d.pair_off = place[u];
+    d.n = XTERMS * d.gsz;
+    d.sbs = d.gsz * XT_STAGE;
+    d.ab_off = place[u] * abs;
+    d.shared = 0;
+    d.pad = 0;
+    gs[g] = d;
+    atomicMax(&hdr->b_max, d.sbs);
+    if (place[u] + d.gsz == valid) {                      // the last group of the call
+      hdr->n_groups = g + 1;
+      hdr->n_pairs = valid;
+    }
   }
 }

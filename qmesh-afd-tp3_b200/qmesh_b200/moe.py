@@ -1,6 +1,6 @@
 """A whole MoE layer for a few tokens (qx_moe_decode_tc): the router's product, the
-top-k selection, the NVFP4 routed experts over a column range and a shared expert,
-as two kernels.
+top-k selection, the NVFP4 routed experts over a column range and a shared expert in
+one call.
 
     out = moe_layer(arena, li, x, gate, topk=6, shared=shared_arena.view(0))
 

@@ -286,9 +286,8 @@ int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* args, con
                               const QxXchgArgs* x, void* stream);
 
 /* ---- a whole MoE layer for a few tokens ----------------------------------------
- * The router's product in front of the tensor-core slice: a router kernel beside
- * the slice's own prologue, and the slice, which selects the experts itself (the
- * reference takes ids and weights from its serving engine's router,
+ * The router's product and the selection in front of the tensor-core slice, beside
+ * the slice's own prologue (the reference takes ids and weights from its serving engine's router,
  * afd_session.py:211-252; no counterpart there):
  *   l[r, e] = sum_k x[r, k] gate[e, k] (+ bias[e])          FP32 sums
  *   ids[r]  = the topk experts of the largest l (larger first, lower id first

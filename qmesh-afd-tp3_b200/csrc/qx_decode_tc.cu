@@ -57,10 +57,10 @@
 //                      tile's counter is complete, or hands them to the fused rank
 //                      combine (qx_xchg.cuh).
 //
-// A whole MoE layer (qx_moe_decode_tc) is the same with the router in front:
-// moe_router_kernel computes the logits while moe_prep_kernel computes the x terms,
-// and every CTA of tc_decode_kernel<true> selects the top-k from the logits itself
-// before it builds the routing tables.
+// A whole MoE layer (qx_moe_decode_tc) is the same with the router in front
+// (qx_router.cuh): moe_router_kernel computes the logits, moe_prep_kernel beside it the
+// x terms and, once the logits are there, the selection; tc_decode_kernel<true> then
+// builds the routing tables from that.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
@@ -221,8 +221,9 @@ struct Params {
   float* tw_out;
   const float* addend;    // optional FP32 [rows][HID] added before the output's rounding
   int64_t addend_stride;
-  int sel_off;            // shared-memory offset of the selected ids [P], then weights [P]
-  int sel_warps;          // warps that select: their keys fit the ring
+  int32_t* sel_ids;       // [P] selected experts and weights, written by moe_prep_kernel
+  float* sel_tw;
+  int sel_off;            // their shared-memory offset: ids [P], then weights [P]
 };
 
 struct ItemMeta {
@@ -1012,7 +1013,7 @@ __device__ __forceinline__ bool second_acc(const ItemMeta& m) { return m.nst > 1
 // row 4 rb + et / 32: bf16(sum over slots j in order of y[row * topk + j][k]),
 // a slot without a valid expert adding 0. Returns the 4 BF16 values (zeros for a
 // row past the post's last).
-// `sel`: the call's ids in shared memory, or null (as load_ids). unit_sum is the
+// `sel`: the call's ids in shared memory, or null. unit_sum is the
 // FP32 sum before the rounding.
 __device__ __forceinline__ float4 unit_sum(const Params& p, const int32_t* sel, int tile, int rb, int et, int& row,
                                            int& k) {
@@ -1487,10 +1488,13 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     mbar_wait_bounded(&S.init_bar, 0, &S.mma_scratch[0], 1u, globaltimer_ns() + p.timeout_ns);
   }
   if constexpr (MOE) {
-    // The logits are the front kernel's: wait for it, then select every row's
-    // experts (each CTA all rows, a warp per row; CTA 0 also writes them out).
+    // The kernels in front have selected: ids and weights into shared memory, then
+    // the tables from them.
     pdl_wait();
-    select_rows(p, reinterpret_cast<uint32_t*>(ring), sel, reinterpret_cast<float*>(sel + p.P), warp, p.sel_warps);
+    for (int q = threadIdx.x; q < p.P; q += NTHR) {
+      sel[q] = __ldcg(&p.sel_ids[q]);
+      reinterpret_cast<float*>(sel + p.P)[q] = __ldcg(&p.sel_tw[q]);
+    }
     __syncthreads();
     route_pairs(p, sel, reinterpret_cast<uint32_t*>(ring), gs, ps, &S.hdr);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after this use of it
@@ -1609,7 +1613,8 @@ size_t qx_slice_workspace_tc_bytes(int32_t rows, int32_t topk, int32_t c0, int32
 size_t qx_moe_workspace_bytes(int32_t rows, int32_t n_experts, int32_t topk, int32_t c0, int32_t c1) {
   const size_t n = qx_slice_workspace_tc_bytes(rows, topk, c0, c1);
   if (n == 0 || n_experts < 1 || n_experts > MAXE || topk > n_experts) return 0;
-  return n + (size_t)RSPLIT * rows * ((n_experts + 3) & ~3) * sizeof(float);   // the slice's, then the logits
+  // the slice's, then the logits, the selected ids and weights
+  return n + (size_t)RSPLIT * rows * ((n_experts + 3) & ~3) * sizeof(float) + (size_t)rows * topk * 8;
 }
 
 }  // extern "C"
@@ -1710,8 +1715,6 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
   p.ring_bytes = (int)(SMEM_LIMIT - (size_t)p.ring_off);
   if (p.ring_bytes - 512 < 2 * (A_STAGE + p.bst)) return QX_ERR_SHAPE;   // two slots of the widest group
   p.ns = p.b_off = 0;
-  p.sel_warps = p.ring_bytes / (((arena->n_experts + 3) & ~3) * 4);
-  if (p.sel_warps > NTHR / 32) p.sel_warps = NTHR / 32;
   p.timeout_ns = timeout_ns();
   p.dep_extra = dep_extra();
   // With the clamp, |act| = |silu(min(g, L)) * clamp(u, -L, L)| <= L^2: one
@@ -1770,6 +1773,8 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
     p.sNT = (p.sW + 63) / 64;
   }
   p.logits = nullptr;
+  p.sel_ids = nullptr;
+  p.sel_tw = nullptr;
   p.gate = nullptr;
   p.gate_stride = p.addend_stride = 0;
   p.gate_bias = p.addend = nullptr;
@@ -1779,6 +1784,8 @@ static int tc_launch(const QxArena* arena, const QxSliceArgs* a, const QxXchgArg
     p.ids = nullptr;
     p.tw = nullptr;
     p.logits = reinterpret_cast<float*>(ws + L.total);
+    p.sel_ids = reinterpret_cast<int32_t*>(p.logits + (size_t)RSPLIT * p.rows * logit_row(p));
+    p.sel_tw = reinterpret_cast<float*>(p.sel_ids + p.P);
     p.gate = rt->gate;
     p.gate_stride = rt->gate_stride;
     p.gate_bias = rt->bias;

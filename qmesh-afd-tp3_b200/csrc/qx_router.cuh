@@ -17,7 +17,7 @@ constexpr int RE = 8, RR = 16, RWARPS = PREP_THR / 32, RSPLIT = 4, RK = HID / RS
 static_assert(RK % 32 == 0, "whole blocks of K per warp");
 
 // Floats between the quarters' logits, [rows][E rounded up to 4] each.
-__device__ __forceinline__ int logit_row(const Params& p) { return (p.E + 3) & ~3; }
+__host__ __device__ __forceinline__ int logit_row(const Params& p) { return (p.E + 3) & ~3; }
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -119,42 +119,6 @@ __device__ __forceinline__ void router_unit(const Params& p, int e0, int r0, int
   }
 }
 
-// CTAs: one per (8 experts, 16 rows, quarter of K).
-template <int GT>
-__global__ void __launch_bounds__(PREP_THR) moe_router_kernel(Params p) {
-  pdl_launch_dependents();
-  const int ne = (p.E + RE - 1) / RE, u = blockIdx.x, tile = u / RSPLIT;
-  router_unit<GT>(p, tile % ne * RE, tile / ne * RR, u % RSPLIT);
-}
-
-// The x terms beside the router: started with it (everything the call reads is
-// complete then) and ended after it, so that waiting for this kernel is waiting for
-// both. (One kernel for both ran the units at the router's registers: 13 us against
-// 7 with 48 rows.)
-__global__ void __launch_bounds__(PREP_THR) moe_prep_kernel(Params p) {
-  pdl_launch_dependents();
-  prep_unit(p, blockIdx.x, gridDim.x, false);
-  pdl_wait();
-}
-
-static cudaError_t front_launch(const Params& p, int gate_type, cudaStream_t st) {
-  const int grid = (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR) * RSPLIT;
-  if (gate_type == QX_T_BF16) moe_router_kernel<QX_T_BF16><<<grid, PREP_THR, 0, st>>>(p);
-  else moe_router_kernel<QX_T_F32><<<grid, PREP_THR, 0, st>>>(p);
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return err;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows * NXCH, 1, 1);
-  cfg.blockDim = dim3(PREP_THR, 1, 1);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, moe_prep_kernel, p);
-}
-
 // ------------------------------------------------------------------ selection
 // A logit as an unsigned key in its order: NaN above everything, -0 equal to +0.
 constexpr uint32_t KEY_NEG_INF = 0x007fffffu;
@@ -188,9 +152,9 @@ struct Top2 {
 // the lanes (the lowest id of equals), and a lane that has given both looks through
 // its keys again. Short loops rather than unrolled ones: every SM fetches this code
 // cold, once per call. `l`: the row's logits of the first quarter of K, the others'
-// `step` floats apart. Slot j's id and weight go to ids[j], tw[j].
-__device__ void select_row(const float* l, size_t step, int E, int topk, int lane, uint32_t* keys, int32_t* ids,
-                           float* tw) {
+// `step` floats apart. Lane j returns slot j's id and weight.
+__device__ void select_row(const float* l, size_t step, int E, int topk, int lane, uint32_t* keys, int& id_out,
+                           float& w_out) {
   Top2 best;
 #pragma unroll 3
   for (int e = 4 * lane; e < E; e += 128) {
@@ -228,77 +192,130 @@ __device__ void select_row(const float* l, size_t step, int E, int topk, int lan
   float sum = 0.f;
 #pragma unroll 1
   for (int j = 0; j < topk; ++j) sum += __shfl_sync(0xffffffffu, w, j);
-  if (lane < topk) {
-    ids[lane] = my_id;
-    tw[lane] = my_id >= 0 ? w / sum : 0.f;
+  id_out = my_id;
+  w_out = my_id >= 0 ? w / sum : 0.f;
+}
+
+// ------------------------------------------------------------------ kernels in front
+// CTAs: one per (8 experts, 16 rows, quarter of K).
+template <int GT>
+__global__ void __launch_bounds__(PREP_THR) moe_router_kernel(Params p) {
+  pdl_launch_dependents();
+  const int ne = (p.E + RE - 1) / RE, u = blockIdx.x, tile = u / RSPLIT;
+  router_unit<GT>(p, tile % ne * RE, tile / ne * RR, u % RSPLIT);
+}
+
+// Started with the router (everything the call reads is complete then): the first CTAs
+// wait for its logits and select, a warp per row; the others compute the x terms
+// meanwhile. (Selecting in every CTA of the decode kernel took 11 us with 48 rows;
+// x terms in the router's kernel ran at its registers, 13 us against 7.)
+// A CTA selects as many rows (8 at most) as their keys fit 24 KB of shared memory.
+constexpr int SEL_BYTES = 24576;
+__host__ __device__ __forceinline__ int select_per_cta(const Params& p) {
+  const int fit = SEL_BYTES / (((p.E + 3) & ~3) * 4);
+  return fit < RWARPS ? fit : RWARPS;
+}
+__global__ void __launch_bounds__(PREP_THR) moe_prep_kernel(Params p, int nsel) {
+  pdl_launch_dependents();
+  if ((int)blockIdx.x >= nsel) {
+    prep_unit(p, blockIdx.x - nsel, gridDim.x - nsel, false);
+    return;
+  }
+  __shared__ __align__(16) uint32_t keys[SEL_BYTES / 4];   // a row of logits per warp
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E4 = logit_row(p);
+  const int per = select_per_cta(p), r = blockIdx.x * per + warp;
+  if (warp >= per || r >= p.rows) return;
+  int id;
+  float w;
+  select_row(p.logits + (size_t)r * E4, (size_t)p.rows * E4, p.E, p.topk, lane, keys + warp * E4, id, w);
+  if (lane < p.topk) {
+    const int q = r * p.topk + lane;
+    p.sel_ids[q] = id;
+    p.sel_tw[q] = w;
+    if (p.ids_out) p.ids_out[q] = id;
+    if (p.tw_out) p.tw_out[q] = w;
   }
 }
 
-// Every row of the call into shared memory (ids[P], tw[P]), a warp per row; `keys`:
-// E4 words per warp.
-__device__ void select_rows(const Params& p, uint32_t* keys, int32_t* ids, float* tw, int warp, int warps) {
-  const int lane = threadIdx.x & 31, E4 = logit_row(p);
-  if (warp >= warps) return;
-#pragma unroll 1
-  for (int r = warp; r < p.rows; r += warps) {
-    int32_t* ir = ids + r * p.topk;
-    float* wr = tw + r * p.topk;
-    select_row(p.logits + (size_t)r * E4, (size_t)p.rows * E4, p.E, p.topk, lane, keys + warp * E4, ir, wr);
-    if (blockIdx.x == 0 && lane < p.topk) {
-      if (p.ids_out) p.ids_out[r * p.topk + lane] = ir[lane];
-      if (p.tw_out) p.tw_out[r * p.topk + lane] = wr[lane];
-    }
-  }
+static cudaError_t front_launch(const Params& p, int gate_type, cudaStream_t st) {
+  const int grid = (p.E + RE - 1) / RE * ((p.rows + RR - 1) / RR) * RSPLIT;
+  if (gate_type == QX_T_BF16) moe_router_kernel<QX_T_BF16><<<grid, PREP_THR, 0, st>>>(p);
+  else moe_router_kernel<QX_T_F32><<<grid, PREP_THR, 0, st>>>(p);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  const int per = select_per_cta(p), nsel = (p.rows + per - 1) / per;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(nsel + p.rows * NXCH, 1, 1);
+  cfg.blockDim = dim3(PREP_THR, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, moe_prep_kernel, p, nsel);
 }
 
+// ------------------------------------------------------------------ routing tables
 // The routing tables of route_sort (unique experts ascending, an expert's pairs in
 // order, split evenly into groups of at most gmax) from the ids in shared memory, by
-// all threads of the CTA instead of one warp: a pair's place, its expert's first place
-// and pair count are counts over all pairs, a group's number a sum over the places
-// before its expert's. `scratch`: 2 MAXP words. (In one warp, sorting network and
-// scans took 41 us for 288 pairs.)
+// all threads of the CTA instead of one warp: a pair's place is the number of smaller
+// keys (expert << 9 | pair), its run's ends are found by walking the sorted keys, a
+// group's number is a sum over the places before its run. `scratch`: 3 MAXP words. (In
+// one warp, sorting network and scans took 41 us for 288 pairs.)
 __device__ void route_pairs(const Params& p, const int32_t* ids, uint32_t* scratch, GroupS* gs, PairS* ps,
                             RouteHdr* hdr) {
-  constexpr uint32_t NONE = 0xffffffffu;
-  constexpr int PT = (MAXP + NTHR - 1) / NTHR;            // pairs per thread
+  constexpr uint32_t NONE = 0xffffffffu;                  // no expert: after every key
+  constexpr int PT = (MAXP + NTHR - 1) / NTHR;            // pairs (then places) per thread
   const int P4 = (p.P + 3) & ~3, gmax = min(GMAX, p.rows), tid = threadIdx.x;
-  uint32_t *keys = scratch, *runs = scratch + MAXP;       // runs: at an expert's first place, its groups
+  uint32_t *keys = scratch, *sorted = scratch + MAXP, *runs = scratch + 2 * MAXP;   // runs: groups, at a run's start
+  int mine = 0;                                           // this thread's pairs with an expert
   for (int i = tid; i < P4; i += NTHR) {
-    keys[i] = i < p.P && ids[i] >= 0 ? (uint32_t)ids[i] << 9 | (uint32_t)i : NONE;
+    const bool has = i < p.P && ids[i] >= 0;
+    keys[i] = has ? (uint32_t)ids[i] << 9 | (uint32_t)i : NONE;
+    sorted[i] = NONE;
     runs[i] = 0u;
+    mine += has;
   }
   if (tid == 0) hdr->n_groups = hdr->n_pairs = hdr->b_max = 0;
   __syncthreads();
-  int place[PT], start[PT], count[PT], valid = 0;
+  if (mine) atomicAdd(&hdr->n_pairs, mine);
+  for (int i = tid; i < p.P; i += NTHR) {
+    const uint32_t k = keys[i];
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < P4; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(keys + j);
+      place += (int)(o.x < k) + (int)(o.y < k) + (int)(o.z < k) + (int)(o.w < k);
+    }
+    if (k != NONE) sorted[place] = k;
+  }
+  __syncthreads();
+  const int valid = hdr->n_pairs;
+  int start[PT], count[PT];
 #pragma unroll
   for (int u = 0; u < PT; ++u) {
     const int i = tid + u * NTHR;
-    place[u] = -1;
-    if (i >= p.P || keys[i] == NONE) continue;
-    const uint32_t k = keys[i], lo = k & ~511u, hi = k | 511u;   // the expert's keys lie in [lo, hi]
-    int below = 0, before = 0, upto = 0;
-    valid = 0;
-#pragma unroll 2
-    for (int j = 0; j < P4; j += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(keys + j);
-      below += (int)(o.x < lo) + (int)(o.y < lo) + (int)(o.z < lo) + (int)(o.w < lo);
-      before += (int)(o.x < k) + (int)(o.y < k) + (int)(o.z < k) + (int)(o.w < k);
-      upto += (int)(o.x <= hi) + (int)(o.y <= hi) + (int)(o.z <= hi) + (int)(o.w <= hi);
-      valid += (int)(o.x != NONE) + (int)(o.y != NONE) + (int)(o.z != NONE) + (int)(o.w != NONE);
-    }
-    place[u] = before;
-    start[u] = below;
-    count[u] = upto - below;
-    ps[before].pq = i;
-    ps[before].row = div_small(i, p.topk);
-    if (before == below) runs[below] = (uint32_t)div_small(count[u] + gmax - 1, gmax);
+    start[u] = count[u] = 0;
+    if (i >= valid) continue;
+    const uint32_t k = sorted[i], e = k >> 9;
+    int a = i, b = i + 1;
+    while (a > 0 && sorted[a - 1] >> 9 == e) --a;
+    while (b < valid && sorted[b] >> 9 == e) ++b;
+    start[u] = a;
+    count[u] = b - a;
+    ps[i].pq = (int)(k & 511u);
+    ps[i].row = div_small((int)(k & 511u), p.topk);
+    if (a == i) runs[i] = (uint32_t)div_small(b - a + gmax - 1, gmax);
   }
   __syncthreads();
   const int abs = ((p.NT + SK - 1) / SK) * XT_STAGE;      // down-operand bytes per pair
 #pragma unroll
   for (int u = 0; u < PT; ++u) {
-    if (place[u] < 0) continue;
-    const int c = count[u], r = place[u] - start[u], ng = div_small(c + gmax - 1, gmax);
+    const int i = tid + u * NTHR, c = count[u];
+    if (c == 0) continue;
+    const int r = i - start[u], ng = div_small(c + gmax - 1, gmax);
     const int gk = div_small((r + 1) * ng - 1, c);        // the k with k c / ng <= r < (k + 1) c / ng
     const int lo = div_small(gk * c, ng);
     if (r != lo) continue;                                // the group's first pair writes its record
@@ -309,19 +326,16 @@ __device__ void route_pairs(const Params& p, const int32_t* ids, uint32_t* scrat
            (j + 3 < start[u] ? (int)o.w : 0);
     }
     GroupS d;
-    d.expert = (int)(keys[tid + u * NTHR] >> 9);
+    d.expert = (int)(sorted[i] >> 9);
     d.gsz = div_small((gk + 1) * c, ng) - lo;
-    d.pair_off = place[u];
+    d.pair_off = i;
     d.n = XTERMS * d.gsz;
     d.sbs = d.gsz * XT_STAGE;
-    d.ab_off = place[u] * abs;
+    d.ab_off = i * abs;
     d.shared = 0;
     d.pad = 0;
     gs[g] = d;
     atomicMax(&hdr->b_max, d.sbs);
-    if (place[u] + d.gsz == valid) {                      // the last group of the call
-      hdr->n_groups = g + 1;
-      hdr->n_pairs = valid;
-    }
+    if (i + d.gsz == valid) hdr->n_groups = g + 1;        // the last group of the call
   }
 }

@@ -45,7 +45,7 @@ def test_refusals(lib):
     assert _call(lib, x_fmt=_lib.QX_X_E4M3, x_scale=0) == _lib.QX_ERR_ARG
     assert _call(lib, workspace_bytes=lib.qx_slice_workspace_tc_bytes(2, 6, 0, 256)) == _lib.QX_ERR_WORKSPACE
     need = lib.qx_moe_workspace_bytes(2, 8, 6, 0, 256)
-    assert need == lib.qx_slice_workspace_tc_bytes(2, 6, 0, 256) + 4 * 2 * 8 * 4
+    assert need == lib.qx_slice_workspace_tc_bytes(2, 6, 0, 256) + 4 * 2 * 8 * 4 + 2 * 6 * 8
     assert lib.qx_moe_workspace_bytes(2, 5, 6, 0, 256) == lib.qx_moe_workspace_bytes(65, 8, 6, 0, 256) == 0
 
 

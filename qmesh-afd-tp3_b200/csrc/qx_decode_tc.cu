@@ -1434,6 +1434,15 @@ __device__ void epilogue(const Params& p, Smem& S, float* xg, const GroupS* gs, 
   }
 }
 
+// This CTA's share of a run of memory (16-byte aligned, a multiple of 16 bytes) towards L2.
+__device__ void prefetch_share(const uint8_t* base, size_t bytes) {
+  constexpr size_t PIECE = 16384;
+  for (size_t o = (size_t)blockIdx.x * PIECE; o < bytes; o += (size_t)gridDim.x * PIECE) {
+    const uint32_t n = (uint32_t)(bytes - o < PIECE ? bytes - o : PIECE);
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(base + o), "r"(n) : "memory");
+  }
+}
+
 template <bool MOE>
 __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -1488,6 +1497,12 @@ __global__ void __launch_bounds__(NTHR, 1) tc_decode_kernel(Params p) {
     mbar_wait_bounded(&S.init_bar, 0, &S.mma_scratch[0], 1u, globaltimer_ns() + p.timeout_ns);
   }
   if constexpr (MOE) {
+    // The shared expert's weights do not depend on the routing: they come into L2
+    // while the kernels in front run (each CTA asks for a share).
+    if (threadIdx.x == 96 && p.sNT > 0) {
+      prefetch_share(p.sw13, (size_t)p.sNT * KB1 * A_KB);
+      prefetch_share(p.sw2, (size_t)HT * p.sNT * A_KB);
+    }
     // The kernels in front have selected: ids and weights into shared memory, then
     // the tables from them.
     pdl_wait();

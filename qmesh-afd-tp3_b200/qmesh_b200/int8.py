@@ -58,24 +58,22 @@ def same_device(dev: torch.device, **tensors) -> None:
         raise ValueError(f"the tensors must be on a CUDA device, not on {dev}")
 
 
-def _rows(t: torch.Tensor, name: str) -> None:
-    if t.dim() != 2 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{name} must be [rows, columns] with unit column stride, got {tuple(t.shape)}")
-    if t.shape[1] > _lib.INT8_MAX_K:
-        raise ValueError(f"{name} has {t.shape[1]} columns, at most {_lib.INT8_MAX_K} sum exactly in 32 bits")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows (a tensor of one row may carry any stride)."""
-    rows, cols = t.shape
-    stride = t.stride()[0]
-    return stride if rows > 1 or stride > cols else cols
+def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, columns, elements between rows) of a [rows, columns] tensor with unit
+    column stride (a tensor of one row may carry any row stride)."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{name} must be [rows, columns] with unit column stride, got {tuple(shape)}")
+    rows, cols = shape
+    if cols > _lib.INT8_MAX_K:
+        raise ValueError(f"{name} has {cols} columns, at most {_lib.INT8_MAX_K} sum exactly in 32 bits")
+    return rows, cols, stride[0] if rows > 1 or stride[0] > cols else cols
 
 
 def _scales(t: torch.Tensor, n: int, name: str) -> None:
     if t.dtype != torch.float32:
         raise TypeError(f"{name} must be float32, got {t.dtype}")
-    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or t.numel() != n or (n > 1 and t.stride()[0] != 1):
         raise ValueError(f"{name} must be a contiguous [{n}] tensor, got {tuple(t.shape)}")
 
 
@@ -85,29 +83,35 @@ def padded(k: int) -> int:
     return (k + 15) // 16 * 16
 
 
-def _check_x(x: torch.Tensor, x_scale: torch.Tensor | None) -> int:
-    """The QX_T_* of activations x with their scale (FP8 only)."""
+def _check_x(x: torch.Tensor, x_scale: torch.Tensor | None) -> tuple[int, int, int, int, int, int]:
+    """(rows, columns, row stride, QX_T_*, scale pointer, scale count) of activations x
+    with their scale (FP8 only)."""
     kind = X_TYPES.get(x.dtype)
     if kind is None:
         raise TypeError(f"x must be bf16, fp16, fp32 or e4m3, got {x.dtype}")
-    _rows(x, "x")
-    if kind == _lib.QX_T_E4M3:
-        if x_scale is None:
-            raise TypeError("FP8 activations need x_scale (per row [rows] or per post [1])")
-        if x_scale.dtype != torch.float32:
-            raise TypeError(f"x_scale must be float32, got {x_scale.dtype}")
-        if x_scale.numel() not in (1, x.shape[0]) or not x_scale.is_contiguous():
-            raise ValueError(f"x_scale has {x_scale.numel()} values for {x.shape[0]} rows")
-    elif x_scale is not None:
-        raise TypeError("x_scale goes with FP8 activations only")
-    return kind
+    rows, k, stride = _rows(x, "x")
+    if kind != _lib.QX_T_E4M3:
+        if x_scale is not None:
+            raise TypeError("x_scale goes with FP8 activations only")
+        return rows, k, stride, kind, 0, 0
+    if x_scale is None:
+        raise TypeError("FP8 activations need x_scale (per row [rows] or per post [1])")
+    if x_scale.dtype != torch.float32:
+        raise TypeError(f"x_scale must be float32, got {x_scale.dtype}")
+    if x_scale.numel() not in (1, rows) or not x_scale.is_contiguous():
+        raise ValueError(f"x_scale has {x_scale.numel()} values for {rows} rows")
+    return rows, k, stride, kind, x_scale.data_ptr(), x_scale.numel()
 
 
-def _check_out(out: torch.Tensor, m: int, n: int) -> None:
-    if out.dtype not in OUT_TYPES:
+def _check_out(out: torch.Tensor, m: int, n: int) -> tuple[int, int]:
+    """(row stride, QX_T_*) of an output tensor."""
+    kind = OUT_TYPES.get(out.dtype)
+    if kind is None:
         raise TypeError(f"out must be bf16, fp16 or fp32, got {out.dtype}")
-    if out.shape != (m, n) or (n > 1 and out.stride()[1] != 1):
-        raise ValueError(f"out must be [{m}, {n}] with unit column stride, got {tuple(out.shape)}")
+    shape, stride = out.shape, out.stride()
+    if len(shape) != 2 or shape[0] != m or shape[1] != n or (n > 1 and stride[1] != 1):
+        raise ValueError(f"out must be [{m}, {n}] with unit column stride, got {tuple(shape)}")
+    return stride[0] if m > 1 or stride[0] > n else n, kind
 
 
 def _new_out(m: int, n: int, dtype: torch.dtype, dev) -> torch.Tensor:
@@ -121,9 +125,8 @@ def quant_int8(x: torch.Tensor, x_scale: torch.Tensor | None = None, q: torch.Te
     """(q int8 [rows, k], scale float32 [rows]): x[r] ~ q[r] * scale[r], the largest
     |x| of a row at +-127. A fresh `q` has its rows 16-byte aligned. A row with a NaN
     or an infinity gets q = 0 and scale = NaN, and is reported by `device_status`."""
-    kind = _check_x(x, x_scale)
+    rows, k, stride, kind, scale_ptr, n_scale = _check_x(x, x_scale)
     dev = x.device
-    rows, k = x.shape
     same_device(dev, x_scale=x_scale, q=q, scale=scale)
     if q is None:
         q = torch.empty(rows, padded(k), dtype=torch.int8, device=dev)[:, :k]
@@ -131,36 +134,32 @@ def quant_int8(x: torch.Tensor, x_scale: torch.Tensor | None = None, q: torch.Te
         scale = torch.empty(rows, dtype=torch.float32, device=dev)
     if q.dtype != torch.int8:
         raise TypeError(f"q must be int8, got {q.dtype}")
-    _rows(q, "q")
-    if q.shape != x.shape:
+    q_rows, q_k, q_stride = _rows(q, "q")
+    if q_rows != rows or q_k != k:
         raise ValueError(f"q is {tuple(q.shape)}, x {tuple(x.shape)}")
     _scales(scale, rows, "scale")
-    launch_on(dev, _lib.load().qx_quant_int8, "qx_quant_int8", x.data_ptr(), _row_stride(x), kind,
-              x_scale.data_ptr() if x_scale is not None else 0, x_scale.numel() if x_scale is not None else 0,
-              rows, k, q.data_ptr(), _row_stride(q), scale.data_ptr())
+    launch_on(dev, _lib.load().qx_quant_int8, "qx_quant_int8", x.data_ptr(), stride, kind, scale_ptr, n_scale, rows, k,
+              q.data_ptr(), q_stride, scale.data_ptr())
     return q, scale
 
 
 def _product(q, scale, w, w_scale, out, out_dtype, swiglu, limit) -> torch.Tensor:
     if q.dtype != torch.int8 or w.dtype != torch.int8:
         raise TypeError(f"q and w must be int8, got {q.dtype}/{w.dtype}")
-    _rows(q, "q")
-    _rows(w, "w")
-    dev = q.device
-    m, k = q.shape
-    wn, wk = w.shape
+    m, k, q_stride = _rows(q, "q")
+    wn, wk, w_stride = _rows(w, "w")
     if wn < 1 or wk != k or (swiglu and wn % 2):
         raise ValueError(f"shape mismatch: q {tuple(q.shape)} w {tuple(w.shape)}")
     n = wn // 2 if swiglu else wn
     _scales(scale, m, "scale")
     _scales(w_scale, wn, "w_scale")
+    dev = q.device
     same_device(dev, scale=scale, w=w, w_scale=w_scale, out=out)
     if out is None:
         out = _new_out(m, n, out_dtype, dev)
-    _check_out(out, m, n)
-    args = _lib.QxInt8Args(q.data_ptr(), _row_stride(q), scale.data_ptr(), w.data_ptr(), _row_stride(w),
-                           w_scale.data_ptr(), out.data_ptr(), _row_stride(out), OUT_TYPES[out.dtype], m, n, k,
-                           1 if swiglu else 0, 1 if swiglu and limit > 0 else 0, float(max(limit, 0.0)))
+    out_stride, kind = _check_out(out, m, n)
+    args = _lib.QxInt8Args(q.data_ptr(), q_stride, scale.data_ptr(), w.data_ptr(), w_stride, w_scale.data_ptr(),
+                           out.data_ptr(), out_stride, kind, m, n, k, swiglu, swiglu and limit > 0, max(limit, 0.0))
     launch_on(dev, _lib.load().qx_int8_matmul, "qx_int8_matmul", ctypes.byref(args))
     return out
 
@@ -201,8 +200,7 @@ class Int8Expert:
                  swiglu_limit: float = SWIGLU_LIMIT):
         if w13.dtype != torch.int8 or w2.dtype != torch.int8:
             raise TypeError(f"w13 and w2 must be int8, got {w13.dtype}/{w2.dtype}")
-        _rows(w13, "w13")
-        _rows(w2, "w2")
+        w13_stride, w2_stride = _rows(w13, "w13")[2], _rows(w2, "w2")[2]
         if w13.shape[0] % 2 or w13.shape[0] < 2 or w2.shape != (w13.shape[1], w13.shape[0] // 2):
             raise ValueError(f"shape mismatch: w13 {tuple(w13.shape)} w2 {tuple(w2.shape)}")
         _scales(w13_scale, w13.shape[0], "w13_scale")
@@ -212,6 +210,7 @@ class Int8Expert:
             if t.device != self.dev:
                 raise ValueError(f"{name} is on {t.device}, not on {self.dev}")
         self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
+        self.weights = (w13.data_ptr(), w13_stride, w13_scale.data_ptr(), w2.data_ptr(), w2_stride, w2_scale.data_ptr())
         self.k, self.inter = w13.shape[1], w13.shape[0] // 2
         self.limit = float(max(swiglu_limit, 0.0))
 
@@ -232,23 +231,19 @@ class Int8Expert:
                  workspace: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """[rows, k] of `out`'s type (or out_dtype) for x [rows, k] (bf16, fp16, fp32, or
         e4m3 with x_scale)."""
-        kind = _check_x(x, x_scale)
-        rows, k = x.shape
+        rows, k, stride, kind, scale_ptr, n_scale = _check_x(x, x_scale)
         if k != self.k:
             raise ValueError(f"x must be [rows, {self.k}], got {tuple(x.shape)}")
         same_device(self.dev, x=x, x_scale=x_scale, out=out, workspace=workspace)
         if out is None:
             out = _new_out(rows, k, out_dtype, self.dev)
-        _check_out(out, rows, k)
+        out_stride, out_kind = _check_out(out, rows, k)
         if workspace is None:
             workspace = self.alloc_workspace(rows)
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
             raise TypeError("workspace must be a contiguous uint8 tensor (alloc_workspace)")
         args = _lib.QxInt8ExpertArgs(
-            x.data_ptr(), _row_stride(x), kind, x_scale.numel() if x_scale is not None else 0,
-            x_scale.data_ptr() if x_scale is not None else 0, self.w13.data_ptr(), _row_stride(self.w13),
-            self.w13_scale.data_ptr(), self.w2.data_ptr(), _row_stride(self.w2), self.w2_scale.data_ptr(),
-            out.data_ptr(), _row_stride(out), OUT_TYPES[out.dtype], rows, k, self.inter, 1 if self.limit > 0 else 0,
-            self.limit, workspace.data_ptr(), workspace.numel())
+            x.data_ptr(), stride, kind, n_scale, scale_ptr, *self.weights, out.data_ptr(), out_stride, out_kind, rows,
+            k, self.inter, self.limit > 0, self.limit, workspace.data_ptr(), workspace.numel())
         launch_on(self.dev, _lib.load().qx_int8_expert, "qx_int8_expert", ctypes.byref(args))
         return out

@@ -230,7 +230,8 @@ def _expert(seed, k, inter):
 
 @pytest.mark.parametrize("rows,k,inter,dtype", [(1, 5120, 64, torch.bfloat16), (6, 640, 288, torch.bfloat16),
                                                 (13, 500, 111, torch.float16), (150, 256, 130, torch.float32),
-                                                (333, 320, 192, torch.bfloat16)])
+                                                (333, 320, 192, torch.bfloat16), (16, 1000, 111, torch.float16),
+                                                (5, 324, 130, torch.float32), (17, 640, 96, torch.bfloat16)])
 def test_expert(cuda_ready, rows, k, inter, dtype):
     """The whole expert equals its four parts called one by one, and is within a bound of
     the 64-bit chain: h differs by at most its relative bound, so h's quantised value can
@@ -261,6 +262,66 @@ def test_expert(cuda_ready, rows, k, inter, dtype):
     err = (out.cpu().double() - want).abs()
     tol = slack + (want.abs() + slack) * (D + rel.amax(1, keepdim=True) + 2 * U)
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("rows", [1, 7, 16, 40])
+def test_expert_fp8_rows_strides_and_nan_rows(cuda_ready, rows):
+    """The expert on the slice's FP8 rows, on strided rows, and with a NaN row, against its
+    four parts; a row that is not finite is NaN, is reported, and leaves the others alone."""
+    from qmesh_b200 import _lib
+    from qmesh_b200.int8 import Int8Expert, device_status, int8_matmul, int8_swiglu, quant_int8
+    w13, w2 = _expert(2, 336, 80)
+    ex = Int8Expert.from_weights(w13.cuda(), w2.cuda(), swiglu_limit=3.0)
+
+    def parts(x, xs=None):
+        h = int8_swiglu(*quant_int8(x, xs), ex.w13, ex.w13_scale, swiglu_limit=3.0, out_dtype=torch.float32)
+        return int8_matmul(*quant_int8(h), ex.w2, ex.w2_scale, out_dtype=torch.float32)
+
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 336, generator=g)
+    x8 = (x * 30).to(torch.float8_e4m3fn).cuda()
+    device_status()
+    for xs in (torch.rand(rows, generator=g).cuda() + 0.1, torch.rand(1, generator=g).cuda() + 0.1):
+        assert torch.equal(ex(x8, xs, out_dtype=torch.float32), parts(x8, xs))
+    wide = torch.zeros(rows, 400, device="cuda")
+    for lead in (0, 4, 3):
+        view = wide[:, lead:lead + 336]
+        view.copy_(x)
+        assert torch.equal(ex(view, out_dtype=torch.float32), parts(view))
+    assert device_status() == 0
+    clean = ex(x.cuda())
+    x[rows // 2, 5] = float("inf")
+    out = ex(x.cuda())
+    assert device_status() == _lib.QX_DEV_NONFINITE
+    keep = torch.arange(rows) != rows // 2
+    assert out[rows // 2].isnan().all() and torch.equal(out[keep], clean[keep])
+
+
+def test_expert_after_its_weights_are_written(cuda_ready):
+    """Weights that the work right in front of the call writes: the call's copies must not
+    run ahead of it (a captured chain: quantise the weights, then the expert)."""
+    from qmesh_b200.int8 import Int8Expert, quant_int8
+    for rows in (4, 40, 300):
+        w = [_expert(s, 2048, 512) for s in (1, 2)]
+        w13, w2 = w[0][0].cuda(), w[0][1].cuda()
+        q13, s13 = quant_int8(w13)
+        q2, s2 = quant_int8(w2)
+        ex = Int8Expert(q13, s13, q2, s2)
+        x = torch.randn(rows, 2048, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+        out, ws = torch.empty_like(x), ex.alloc_workspace(rows)
+        ex(x, out=out, workspace=ws)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            quant_int8(w2, q=q2, scale=s2)
+            quant_int8(w13, q=q13, scale=s13)
+            ex(x, out=out, workspace=ws)
+        for a, b in (w[1], w[0], w[1]):
+            w13.copy_(a)
+            w2.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, Int8Expert.from_weights(a.cuda(), b.cuda())(x))
 
 
 def test_expert_graph_streams_and_empty_batch(cuda_ready):

@@ -327,7 +327,8 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  * qx_quant_int8: x [rows, k] of type x_type (row stride x_stride elements) ->
  * q[r, i] = round_half_even(127 x[r, i] / m_r), scale[r] = m_r / 127 with
  * m_r = max(max_i |x[r, i]|, 1e-30). The quotient is rounded exactly for BF16,
- * FP16 and E4M3 inputs; for FP32 after 127 x has been rounded to FP32. QX_T_E4M3:
+ * FP16 and E4M3 inputs; for FP32 it carries a relative error of 2^-24 when it is
+ * rounded. QX_T_E4M3:
  * x = bf16(float(e4m3) x_scale), x_scale one value (n_scale = 1) or one per row
  * (n_scale = rows), as the slice reads it. A row that holds a NaN or an infinity
  * gets q = 0 and scale = NaN (every product with it is NaN; the other rows are

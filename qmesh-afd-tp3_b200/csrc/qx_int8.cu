@@ -99,17 +99,19 @@ __device__ __forceinline__ uint4 load16(const void* x, int64_t off, int k, int n
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// round_half_even(p / m) for p = 127 x, 0 < m, as the low byte of the result: the
-// estimate p * (1 / m), rounded to a whole number by adding 1.5 * 2^23, is at most
-// one off, and p - n m is exact for 8- and 11-bit x (p and n m both fit 24 bits),
-// so one comparison with half of m settles it; BF16 values often sit on the half
-// itself (x = m / 2 gives 63.5), where an inexact quotient would fall to either side.
-__device__ __forceinline__ uint32_t quotient(float p, float m, float rm) {
-  constexpr float MAGIC = 12582912.f;
-  const float y = fmaf(p, rm, MAGIC), d = fmaf(MAGIC - y, m, p), a2 = 2.f * fabsf(d);
-  uint32_t n = __float_as_uint(y);
-  if (a2 >= m && (a2 > m || (n & 1u))) n += d > 0.f ? 1u : ~0u;
-  return n;
+// round_half_even(127 x / m) as the low byte of the result, c = 127 / m rounded: the
+// whole number comes from adding 1.5 * 2^23. BF16 and FP16 values often sit on a half
+// (x = m / 2 gives 63.5), where an inexact quotient falls to either side: x c is within 2
+// units of its last place of the true quotient, a half has at most 8 significant bits,
+// and any other quotient of 8- or 11-bit numbers is at least 1 / (127 * 4094) of itself
+// (16 units) away from one, so rounding x c to 21 bits first restores the halves and
+// moves nothing over one. FP32 values are rounded as they come, at most 2^-24 off.
+template <int T>
+__device__ __forceinline__ uint32_t quotient(float x, float c) {
+  constexpr float WHOLE = 12582912.f;
+  if constexpr (T == QX_T_F32) return __float_as_uint(fmaf(x, c, WHOLE));
+  const uint32_t t = (__float_as_uint(__fmul_rn(x, c)) + 4u) & ~7u;
+  return __float_as_uint(__uint_as_float(t) + WHOLE);
 }
 
 // Largest |x| of one 16-byte piece, as the bits of its type (16-bit types: of one of
@@ -170,8 +172,7 @@ __global__ void __launch_bounds__(QTHR) quant_kernel(const void* x, int64_t xs, 
   for (int i = 0; i < thr / 32; ++i) m = max(m, sm[i]);
   const bool bad = m >= INF_BITS;
   const float mc = fmaxf(__uint_as_float(m), AMAX_FLOOR);
-  const float f = mc > 1e30f ? 0x1p-20f : 1.f;     // 127 x must not overflow: a power of two changes no quotient
-  const float qm = QMAX * f, mf = mc * f, rm = __frcp_rn(mf);
+  const float c = __fdiv_rn(QMAX, mc);
   const uint32_t keep = bad ? 0u : 0xffffffffu;
   if (threadIdx.x == 0) {
     scale[r] = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(mc, QMAX);
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(QTHR) quant_kernel(const void* x, int64_t xs, 
     for (int j = 0; j < E; j += 4) {
       uint32_t n[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) n[i] = quotient(__fmul_rn(v[j + i], qm), mf, rm);
+      for (int i = 0; i < 4; ++i) n[i] = quotient<T>(v[j + i], c);
       o[j / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) & keep;
     }
     if (q_vec && (g + 1) * E <= k) {

@@ -373,7 +373,7 @@ struct Launch {
 void pair_tile(const Args& p, int sms, int* tb, int* bn) {
   const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, chunks = (p.k + (int)KST - 1) / (int)KST;
   const int h = p.swiglu ? 2 : 1, step = 32 * h;
-  *tb = (p.m + 16 * tiles_m - 1) / (16 * tiles_m) * 8;
+  *tb = (p.m + 64 * tiles_m - 1) / (64 * tiles_m) * 32;
   double least = 0;
   for (int b = 256; b >= 64; b -= step) {
     const int64_t tiles = (int64_t)tiles_m * ((p.n + b / h - 1) / (b / h));
@@ -395,12 +395,9 @@ int pair_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
   if (!row_map(&tw, p.w, p.swiglu ? 2ll * p.n : p.n, p.k, p.ws, bn / 2) || !row_map(&ta, p.a, p.m, p.k, p.as, tb))
     return QX_ERR_DEVICE;
   const int spans = bn >= 160 ? 1 : 2;   // from 160 rows on the MMAs of one span outlast the issuing threads' loop
-  // Tiled stores where the output's rows start on 16-byte boundaries, in boxes that do
-  // not reach from a CTA's tokens into the next one's.
-  int tma = tb % 32 ? 8 : 32;
-  if (reinterpret_cast<uintptr_t>(p.out) % 16 || p.os * osz % 16 ||
-      !tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, tma, CU_TENSOR_MAP_SWIZZLE_64B))
-    tma = 0;
+  // Tiled stores where the output's rows start on 16-byte boundaries.
+  const int tma = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.os * osz % 16 == 0 &&
+                  tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, 32, CU_TENSOR_MAP_SWIZZLE_64B);
   return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, PAIR_SMEM, st, 2)(pair_kernel, tw, ta, to, p, tb, bn, spans, tiles_m,
                                                                   (int)tiles, prefetch, tma, wait_limit_ns());
 }

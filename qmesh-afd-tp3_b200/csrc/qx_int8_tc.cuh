@@ -354,9 +354,8 @@ __device__ __forceinline__ bool epilogue_and(bool pred) {
 constexpr int PAIR_BLOCK = 32 * 64;
 
 // Up to 32 tokens (rows) x COLS output columns from column n on, each lane holding its
-// token's values. Rows on 16-byte boundaries: tiled stores of `tma` (8 or 32) tokens,
-// which leave out what lies past the tensor's end; else (tma = 0) element by element,
-// 64 bytes of a row at a time.
+// token's values. Rows on 16-byte boundaries (tma): one tiled store, which leaves out what
+// lies past the tensor's end; else element by element, 64 bytes of a row at a time.
 template <int COLS>
 __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to, uint8_t* stage, int64_t row0, int rows,
                                             int n, const float* v, int tma, int lane) {
@@ -380,10 +379,9 @@ __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) {
-      for (int r = 0; r < min(rows, 32); r += tma)
-        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(to), "r"(n),
-                     "r"((int)row0 + r), "r"(smem_u32(stage) + r * 64)
-                     : "memory");
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(to), "r"(n),
+                   "r"((int)row0), "r"(smem_u32(stage))
+                   : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     return;
@@ -394,7 +392,7 @@ __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to
   uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + row0 * step + (int64_t)(n + c) * OSZ;
   if (n + c < p.n) {
 #pragma unroll 4
-    for (int r = lane / COLS; r < min(rows, 32); r += 32 / COLS) {
+    for (int r = lane / COLS; r < rows; r += 32 / COLS) {
       const uint8_t* from = stage + r * 64 + 16 * ((c * OSZ / 16) ^ ((r >> 1) & 3)) + c * OSZ % 16;
       if constexpr (OSZ == 4) *reinterpret_cast<float*>(out + r * step) = *reinterpret_cast<const float*>(from);
       else *reinterpret_cast<uint16_t*>(out + r * step) = *reinterpret_cast<const uint16_t*>(from);
@@ -428,7 +426,7 @@ constexpr int PAIR_THR = 96 + 32 * PAIR_EPI;         // weight copies, MMAs, epi
 static_assert(PAIR_SMEM + 1536 <= 232448, "with the static part, one SM's memory");
 
 // A pair of CTAs (the cluster) works on tiles of 2 tb tokens x bn weight rows (tb a
-// multiple of 8, at most 128; bn a multiple of 32, of 64 with SwiGLU, at most 256):
+// multiple of 32, at most 128; bn a multiple of 32, of 64 with SwiGLU, at most 256):
 // CTA r holds tokens [tb r, tb (r + 1)) and weight rows [bn/2 r, bn/2 (r + 1)) of the
 // tile in its shared memory and its tokens' accumulators in its TMEM; CTA 0's warp 1
 // issues the MMAs of both (always M = 256: the rows from tb on read whatever follows
@@ -578,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       if (!ok) continue;
       tc::fence_after_sync();
       const uint32_t t0 = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);
-      const int rows = (int)min((int64_t)(tb - q * 32), p.m - row0);       // this warp's tokens, of 32
+      const int rows = q * 32 < tb ? (int)min((int64_t)32, p.m - row0) : 0;   // this warp's tokens
 #pragma unroll 1
       for (int c = 32 * h; rows > 0 && c < cols && n0 + c < p.n; c += 64) {   // the groups' alternate pieces
         int32_t g[32];

@@ -339,7 +339,8 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  * the sum exact in 32 bits, the result rounded once to out_type. With swiglu = 1,
  * w holds n gate rows and then n up rows (w_scale too) and out[i, j] =
  * g / (1 + exp(-g)) * u, with g = min(g, limit) and u = clamp(u, -limit, limit)
- * first if has_limit. Strides in elements. The same bytes come out whatever m and
+ * first if has_limit (the quotient to 2 units of its last
+ * place). Strides in elements. The same bytes come out whatever m and
  * the alignment are; rows of a and w that start on 16-byte boundaries (address
  * and stride) run on the tensor cores, others on a slower path. m = 0 does
  * nothing; out must not overlap the inputs.

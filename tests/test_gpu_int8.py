@@ -5,9 +5,10 @@ Tolerances. A product's value is ((float)sum * scale) * w_scale: the sum is exac
 and the conversion and the two products round once each, at most 2^-24 relative
 apiece, so the FP32 value is within D = 3 * 2^-24 (1 + 2^-22), and the output
 rounding adds eps / 2 of its type. SwiGLU: silu(g) = g / (1 + exp(-g)) changes by
-at most (1 + |g|) times g's relative change; CUDA documents expf within 2 ulp
-(4 * 2^-24 relative), and the sum, quotient and product add 2^-24 each, so
-act is within ((1 + |g|) + 1) D + 7 * 2^-24 before the output rounding.
+at most (1 + |g|) times g's relative change; CUDA documents expf and __fdividef within
+2 ulp each (4 * 2^-24 relative; the divisor is below 2^126 for |g| < 87), and the sum
+and the product add 2^-24 each, so act is within ((1 + |g|) + 1) D + 10 * 2^-24 before
+the output rounding.
 """
 
 import pytest
@@ -182,7 +183,7 @@ def test_swiglu(cuda_ready, m, n, k, limit, pad):
     qa, sa, da, dsa = rows_of(m + n, m, k, 2.0 / k ** 0.5 / 0.02, pad)
     qw, sw, dw, dsw = rows_of(m * 5 + k, 2 * n, k, 0.02, pad)
     g, u, want = ref_swiglu(ref_product(qa, sa, qw, sw), limit)
-    rel = (2 + g.abs()) * D + 7 * U
+    rel = (2 + g.abs()) * D + 10 * U
     for dtype in (torch.float32, torch.bfloat16):
         out = int8_swiglu(da, dsa, dw, dsw, swiglu_limit=limit, out_dtype=dtype)
         close(out, want, rel, dtype)
@@ -250,7 +251,7 @@ def test_expert(cuda_ready, rows, k, inter, dtype):
     assert torch.equal(out, ex(x.cuda(), out_dtype=torch.float32, workspace=ws))
     # the 64-bit chain from the kernel's own q (exact or checked above) on
     g, u, hw = ref_swiglu(ref_product(q.cpu(), s.cpu(), ex.w13.cpu(), ex.w13_scale.cpu()), 10.0)
-    rel = (2 + g.abs()) * D + 7 * U
+    rel = (2 + g.abs()) * D + 10 * U
     assert ((h.cpu().double() - hw).abs() <= (rel + U) * hw.abs() + 1e-42).all()
     m = hw.abs().amax(1, keepdim=True).clamp(min=TINY)
     t = 127.0 * hw / m

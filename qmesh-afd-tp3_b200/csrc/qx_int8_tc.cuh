@@ -123,9 +123,12 @@ __device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
   return ok != 0u;
 }
 
-// Bounded wait: false once the deadline has passed, with QX_DEV_TIMEOUT recorded;
-// the caller then stops consuming.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t deadline) {
+// Bounded wait: false once `limit` ns have passed, with QX_DEV_TIMEOUT recorded; the
+// caller then stops consuming. The time runs from this wait's own start, and no thread
+// waits here for what depends on the kernel in front before that one has ended
+// (pdl_wait), so neither a long product nor a long kernel in front uses it up.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t limit) {
+  const uint64_t deadline = globaltimer_ns() + limit;
   for (uint32_t it = 0;; ++it) {
     if (try_phase(bar, parity)) return true;
     if ((it & 15u) == 15u && globaltimer_ns() > deadline) {
@@ -134,8 +137,8 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t 
     }
   }
 }
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint64_t deadline) {
-  return try_phase(bar, parity) || wait_long(bar, parity, deadline);
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint64_t limit) {
+  return try_phase(bar, parity) || wait_long(bar, parity, limit);
 }
 
 // ---- accumulator loads ---------------------------------------------------------------
@@ -228,7 +231,6 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
   if (warp == 0 && elect_one()) {
     if (!prefetch) pdl_wait();
@@ -236,15 +238,15 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     int s = 0;
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
-      if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+      if (c == c0 + L::NS) pdl_wait();
+      if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
       mbar_arrive_expect_tx(&full[s], L::STAGE);
       tma_2d(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
       if (p.swiglu) tma_2d(base + s * L::STAGE + 64 * KST, &tw, c * (int)KST, p.n + n0, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
     if (!ok) {                                            // copies still in flight land before the CTA leaves
-      const uint64_t grace = globaltimer_ns() + timeout;
-      for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, grace);
+      for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, timeout);
     }
   } else if (warp == 6 && elect_one()) {
     pdl_wait();
@@ -252,15 +254,16 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     int s = 0;
     uint32_t ph = 1;
     for (int c = c0; c < c1; ++c) {
-      if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+      if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
       tma_2d(base + s * L::STAGE, &ta, c * (int)KST, 0, bars + 8 * s);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
   } else if (warp == 1 && elect_one()) {
+    pdl_wait();
     int s = 0;
     uint32_t ph = 0;
     for (int c = c0; c < c1; ++c) {
-      if (!(ok = wait_phase(&full[s], ph, deadline))) break;
+      if (!(ok = wait_phase(&full[s], ph, timeout))) break;
       tc::fence_after_sync();
       const uint64_t da = sdesc128(smem_u32(ring) + s * L::STAGE), db = da + (L::A_BYTES >> 4);
 #pragma unroll
@@ -272,7 +275,8 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   }
   __syncwarp();
   const bool epi = warp >= 2 && warp < 6;
-  if (epi) ok = wait_phase(&done, 0, deadline + timeout);
+  pdl_wait();                                             // also: the tokens' scales, and the output's place
+  if (epi) ok = wait_phase(&done, 0, 2 * timeout);
   cluster_wait();                                         // every CTA of the cluster has started
   if (epi && __all_sync(0xffffffffu, ok)) {
     tc::fence_after_sync();
@@ -293,7 +297,6 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     }
     tc::fence_before_sync();
   }
-  pdl_wait();                                             // the tokens' scales, and the output's place
   cluster_sync();
   if (warp == 1) tc::tmem_dealloc(tmem, L::COLS);
   // items of this CTA: (own token, four weight rows)
@@ -478,7 +481,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   tc::fence_before_sync();
   cluster_sync();
   tc::fence_after_sync();
-  const uint64_t deadline = globaltimer_ns() + timeout;
   bool ok = true;
   if (warp == 0 && elect_one()) {
     const uint32_t bytes = 2 * stage_bytes;               // both CTAs' copies
@@ -492,7 +494,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       const int nt = tile / tiles_m * cols;
       const int n0 = rank == 0 ? nt : p.swiglu ? p.n + nt : nt + bn / 2;
       for (int c = 0; c < stages; ++c) {
-        if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+        if (tile > pair || c >= ns) pdl_wait();
+        if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
         if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
         for (int g = 0; g < spans; ++g)
           tma_2d_pair(base + s * stage_bytes + g * b_span, &tw, c * kst + g * (int)KST, n0, bars + 8 * s);
@@ -502,8 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     // Copies still in flight after a wait that ran out count on CTA 0's barriers;
     // the cluster barrier below holds CTA 1 until CTA 0 has waited for them.
     if (!ok && rank == 0) {
-      const uint64_t grace = globaltimer_ns() + timeout;
-      for (int i = 0; i < ns; ++i) wait_phase(&full[i], 0, grace);
+      for (int i = 0; i < ns; ++i) wait_phase(&full[i], 0, timeout);
     }
   } else if (warp == 2 + PAIR_EPI && elect_one()) {
     pdl_wait();
@@ -513,7 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
       const int m0 = (tile % tiles_m * 2 + (int)rank) * tb;
       for (int c = 0; c < stages; ++c) {
-        if (!(ok = wait_phase(&empty[s], ph, deadline))) break;
+        if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
         for (int g = 0; g < spans; ++g)
           tma_2d_pair(base + s * stage_bytes + g * a_span, &ta, c * kst + g * (int)KST, m0, bars + 8 * s);
         if (++s == ns) s = 0, ph ^= 1;
@@ -521,14 +523,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     }
   } else if (warp == 1 && rank == 0 && elect_one()) {
     const uint32_t idesc = idesc_i8(256, (uint32_t)bn);
+    pdl_wait();
     int s = 0, it = 0;
     uint32_t ph = 0;
     for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
       const int b = it & 1;
-      if (!(ok = wait_phase(&acc_empty[b], ((it >> 1) & 1) ^ 1, deadline))) break;
+      if (!(ok = wait_phase(&acc_empty[b], ((it >> 1) & 1) ^ 1, timeout))) break;
       tc::fence_after_sync();
       for (int c = 0; c < stages; ++c) {
-        if (!(ok = wait_phase(&full[s], ph, deadline))) break;
+        if (!(ok = wait_phase(&full[s], ph, timeout))) break;
         tc::fence_after_sync();
         const uint64_t da = sdesc128(smem_u32(ring) + s * stage_bytes), db = da + (spans * a_span >> 4);
         for (int g = 0; g < spans; ++g) {
@@ -543,7 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       commit_pair(&acc_full[b]);
     }
     commit_pair(&drained);
-    wait_phase(&drained, 0, deadline + timeout);          // no MMA is in flight when TMEM is released
+    wait_phase(&drained, 0, 2 * timeout);          // no MMA is in flight when TMEM is released
   } else if (warp >= 2 && warp < 2 + PAIR_EPI) {
     const int q = warp & 3, et = threadIdx.x - 64, h = warp >= 6;   // lane quarter, thread, warp group
     uint8_t* stage = ring + PAIR_RING + (warp - 2) * 2 * PAIR_BLOCK;
@@ -572,7 +575,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       sws[et] = next_w;
       look_ahead(tile + pairs);
       if (!epilogue_and(ok)) break;                       // this tile's sws are written; a wait that ran out ends all
-      ok = __all_sync(0xffffffffu, wait_phase(&acc_full[b], (it >> 1) & 1, deadline));
+      ok = __all_sync(0xffffffffu, wait_phase(&acc_full[b], (it >> 1) & 1, timeout));
       if (!ok) continue;
       tc::fence_after_sync();
       const uint32_t t0 = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);

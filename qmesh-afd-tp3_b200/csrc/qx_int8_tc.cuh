@@ -614,6 +614,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       if (lane == 0) arrive_cluster(mapa(smem_u32(&acc_empty[b]), 0));
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the stores are in memory
+    // CTA 0's last arrival on this CTA's barriers has come before this CTA may leave.
+    if (rank == 1 && warp == 2 && lane == 0) wait_phase(&drained, 0, 2 * timeout);
   }
   __syncwarp();
   tc::fence_before_sync();

@@ -1,6 +1,6 @@
 // The router of a whole MoE layer, part of qx_decode_tc.cu (included inside its
-// namespace): the logits beside the x terms in moe_front_kernel, the selection of
-// the experts in every CTA of the decode kernel.
+// namespace): the logits (moe_router_kernel), the selection beside the x terms
+// (moe_prep_kernel) and the decode kernel's routing tables from it (route_pairs).
 
 // ------------------------------------------------------------------ logits
 // One CTA: 16 rows x 8 experts over a quarter of K, on warp-level BF16 tensor-core

@@ -309,3 +309,55 @@ def test_prefill_with_int8_shared_expert(cuda_ready):
         routed = prefill_slice(ar, 0, x, ids.to(dev), tw.to(dev), a2, **kw)
         assert torch.equal(got, combine_ordered([routed, ex(x, xs)]))
         assert not torch.equal(got, routed)
+
+
+@pytest.mark.parametrize("rows,n_exp,topk", [(64, 4096, 8), (33, 1501, 8), (1, 4096, 1)])
+def test_many_experts(cuda_ready, rows, n_exp, topk):
+    """The most rows, experts and slots that a call takes: up to 4096 keys per row in
+    shared memory, 512 pairs in the routing tables. The last expert ties with the first."""
+    from qmesh_b200.arena import Arena
+    from qmesh_b200.expert_slice import device_status, expert_slice
+    from qmesh_b200.moe import alloc_workspace, moe_layer
+    dev = cuda_ready
+    ar = Arena(dev, 1, n_exp, 0, 32)
+    ar.fill_synthetic(0, seed=3)
+    x, gate, b = inputs(n_exp, rows, n_exp, torch.bfloat16, True)
+    gate[-1], b[-1] = gate[0], b[0]
+    ids = torch.empty(rows, topk, dtype=torch.int32, device=dev)
+    tw = torch.empty(rows, topk, device=dev)
+    ws = alloc_workspace(rows, n_exp, topk, 0, 32, dev)
+    dx = x.to(dev)
+    out = torch.full((rows + 1, 5120), 3.0, dtype=torch.bfloat16, device=dev)
+    moe_layer(ar, 0, dx, gate.to(dev), bias=b.to(dev), topk=topk, ids=ids, tw=tw, workspace=ws, out=out)
+    assert device_status(ws) == 0
+    l, bound = logits64(x, gate, b)
+    check_selection(ids, tw, l, bound, topk)
+    for r in ids.tolist():
+        assert n_exp - 1 not in r or (0 in r and r.index(0) < r.index(n_exp - 1))
+    assert torch.equal(out[:rows], expert_slice(ar, 0, dx, ids, tw)) and (out[rows] == 3.0).all()
+
+
+def test_two_layers_on_two_streams(cuda_ready):
+    """Two calls at once, each with its own workspace and its own INT8 shared expert
+    workspaces, give the bytes of the calls one after the other."""
+    from qmesh_b200.int8 import Int8Expert
+    from qmesh_b200.moe import alloc_workspace, moe_layer
+    dev = cuda_ready
+    layer = layer_of(14, 16, 96)
+    ar = arena_of(dev, layer, 16, 96)
+    g = torch.Generator().manual_seed(2)
+    ex = Int8Expert.from_weights((torch.randn(192, 5120, generator=g) * 0.02).to(dev),
+                                 (torch.randn(5120, 96, generator=g) * 0.05).to(dev))
+    data = [[t if t is None else t.to(dev) for t in inputs(30 + i, 5 + i, 16, torch.float32, True)] for i in range(2)]
+    want = [moe_layer(ar, 0, x, gate, bias=b, shared=ex) for x, gate, b in data]
+    ws = [alloc_workspace(6, 16, 6, 0, 96, dev) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, gate, b) in enumerate(data):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(moe_layer(ar, 0, x, gate, bias=b, shared=ex, workspace=ws[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])

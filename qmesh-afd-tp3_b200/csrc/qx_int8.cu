@@ -221,9 +221,27 @@ struct Args {
   float limit;
 };
 
-// Any alignment: 64 x 64 sums per CTA by dp4a over 64-byte pieces of K staged in
-// shared memory byte by byte. Serves rows whose address or stride the copy
-// engine cannot take (not a multiple of 16 bytes).
+// 16 bytes of a row from byte address p on, the first n >= 1 of them valid (the others 0):
+// aligned words that overlap the valid bytes, shifted into place.
+__device__ __forceinline__ uint4 load16_any(const int8_t* p, int n) {
+  const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3u);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p - sh);
+  uint32_t v[5], o[4];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) v[j] = 4 * j < (int)sh + n ? __ldcg(w + j) : 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int left = n - 4 * j;                          // valid bytes of this word and those behind it
+    o[j] = __funnelshift_r(v[j], v[j + 1], 8 * sh) & (left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1u);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Any alignment: 64 x 64 sums per CTA by dp4a over 64-byte pieces of K in shared
+// memory, the next piece's loads under way meanwhile. Serves rows whose address or
+// stride the copy engine cannot take (not a multiple of 16 bytes); bound by dp4a's
+// rate (2048 x 5120 x 2303: 669 us against 20.6 for aligned rows) and with few tokens
+// by the latency of its rounds over K (1 x 2222 x 1111: 25 us; byte loads took 76).
 constexpr int ST = 64, SKB = 64;
 __global__ void __launch_bounds__(256) plain_kernel(Args p) {
   __shared__ __align__(16) int8_t sa[ST][SKB + 4], sw[ST][SKB + 4];
@@ -233,15 +251,26 @@ __global__ void __launch_bounds__(256) plain_kernel(Args p) {
   const int half = p.swiglu ? ST / 2 : ST;               // output columns of the tile
   const int n0 = blockIdx.x * half, m0 = blockIdx.y * ST;
   int32_t acc[4][4] = {};                                // tokens ty + 16 i, weight rows tx + 16 j
+  const int r = tid >> 2, c = (tid & 3) * 16;            // this thread's row of both operands, its 16 bytes
+  const int nr = n0 + (r < half ? r : r - half);         // output column of its weight row
+  const int8_t* pa = m0 + r < p.m ? p.a + (int64_t)(m0 + r) * p.as + c : nullptr;
+  const int8_t* pw = nr < p.n ? p.w + (int64_t)(r < half ? nr : p.n + nr) * p.ws + c : nullptr;
+  uint4 va, vw;
+  auto fetch = [&](int k0) {
+    const int left = p.k - k0 - c, n = left < 16 ? left : 16;
+    va = pa && n > 0 ? load16_any(pa + k0, n) : make_uint4(0u, 0u, 0u, 0u);
+    vw = pw && n > 0 ? load16_any(pw + k0, n) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  auto put = [&](int8_t* to, const uint4& v) {
+    uint32_t* t = reinterpret_cast<uint32_t*>(to);
+    t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
+  };
+  fetch(0);
   for (int k0 = 0; k0 < p.k; k0 += SKB) {
-    for (int i = tid; i < ST * SKB; i += 256) {
-      const int r = i / SKB, c = i % SKB;
-      const int wr = r < half ? n0 + r : p.n + n0 + r - half;
-      const bool w_ok = (r < half ? n0 + r : n0 + r - half) < p.n;
-      sa[r][c] = (m0 + r < p.m && k0 + c < p.k) ? p.a[(int64_t)(m0 + r) * p.as + k0 + c] : (int8_t)0;
-      sw[r][c] = (w_ok && k0 + c < p.k) ? p.w[(int64_t)wr * p.ws + k0 + c] : (int8_t)0;
-    }
+    put(&sa[r][c], va);
+    put(&sw[r][c], vw);
     __syncthreads();
+    if (k0 + SKB < p.k) fetch(k0 + SKB);
 #pragma unroll 4
     for (int c = 0; c < SKB; c += 4) {
       int av[4], wv[4];

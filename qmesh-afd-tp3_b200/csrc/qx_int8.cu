@@ -40,9 +40,10 @@ __device__ __forceinline__ float scaled(int32_t sum, float sa, float sw) {
   return __fmul_rn(__fmul_rn(__int2float_rn(sum), sa), sw);
 }
 
-// Comparisons, not fminf: a NaN (a row the quantiser refused) stays one. The quotient
-// is within 2 units of its last place (2^-22); the IEEE division's way for a zero gate
-// cost every tile with one 4 us.
+// Comparisons, not fminf: a NaN (from a row that the quantiser refused) stays one. The
+// quotient is within 2 units of its last place (2^-22), and 0 for gates below -87.3, whose
+// denominator is above 2^126 (the sigmoid is below 2^-126 there); the IEEE division's way
+// for a zero gate cost every tile with one 4 us.
 __device__ __forceinline__ float swiglu(float g, float u, float limit, bool has_limit) {
   if (has_limit) {
     g = g > limit ? limit : g;
@@ -107,7 +108,8 @@ __device__ __forceinline__ uint4 load16(const void* x, int64_t off, int k, int n
 // units of its last place of the true quotient, a half has at most 8 significant bits,
 // and any other quotient of 8- or 11-bit numbers is at least 1 / (127 * 4094) of itself
 // (16 units) away from one, so rounding x c to 21 bits first restores the halves and
-// moves nothing over one. FP32 values are rounded as they come, at most 2^-24 off.
+// moves nothing over one (for m >= AMAX_FLOOR, below which c is not 127 over such a
+// number). FP32 values are rounded as they come, at most 2^-24 off.
 template <int T>
 __device__ __forceinline__ uint32_t quotient(float x, float c) {
   constexpr float WHOLE = 12582912.f;
@@ -138,7 +140,9 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t m, const uint4& raw, float
 
 // One CTA per row, about four 16-byte pieces per thread. The row is read once and
 // kept in registers (raw) between the maximum and the quantisation; what is longer
-// than NV pieces per thread is read again. Bound by the bytes. early: 1 lets the
+// than NV pieces per thread is read again. Bound by the bytes (8192 x 5120 BF16: 24.3 us,
+// 5.2 TB/s; 8192 x 2304 FP32: 17.8 us, 5.3 TB/s; a persistent form, the next row's loads
+// ahead, took 48 us where this one then took 35). early: 1 lets the
 // kernels behind this one start before it has waited for the ones in front (their
 // weights are then known to be complete).
 constexpr int QTHR = 512, NV = 4;
@@ -399,8 +403,8 @@ struct Launch {
 // over the pairs takes, per 128-byte chunk of K, the longer of the MMAs (1.3 ns a weight
 // row) and the copies into one SM (64 bytes a clock: 1.05 ns a row of its operands, 60 ns
 // at least), or an epilogue (1.4 us for 256 rows) if that is longer; the last epilogue
-// comes on top. Measured at 2048 x 5120 x 2304: 18.3 us with 192 rows (3 waves), 20.8 with
-// 256 (3), 22.8 with 128 (5).
+// comes on top. Measured at 2048 x 5120 x 2304: 20.4 us with 224 rows, 20.6 with 192 (which the
+// estimate takes), 21.1 with 256 (each 3 waves), 21.9 with 128 (5).
 void pair_tile(const Args& p, int sms, int* tb, int* bn) {
   const int tiles_m = (p.m + 255) / 256, pairs = sms / 2, chunks = (p.k + (int)KST - 1) / (int)KST;
   const int h = p.swiglu ? 2 : 1, step = 32 * h;
@@ -435,7 +439,7 @@ int pair_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
 
 // K pieces of the split kernel (1..8): the fewest that leave a CTA the least of K while
 // all clusters fit on the GPU at once (two CTAs per SM, less what clusters leave unused of
-// a group of SMs: 1.65 per SM; 5120 x 5120 in 6 pieces takes 9.2 us, in 8 14).
+// a group of SMs: 1.65 per SM; 5120 x 5120 with one token: 8.0 us in 5 pieces, 8.2 in 6, 11.4 in 7).
 int pieces_of(int64_t tiles, int chunks, int sms) {
   int best = 1;
   for (int s = 2; s <= 8 && s <= chunks; ++s)
@@ -465,8 +469,8 @@ int product(Args p, int prefetch, int sms, cudaStream_t st) {
   if (aligned(p.a, p.as, p.m) && aligned(p.w, p.ws, p.swiglu ? 2 : p.n)) {
     if (p.m == 1) p.as = (p.as + 15) / 16 * 16;          // never stepped
     if (p.n == 1 && !p.swiglu) p.ws = (p.ws + 15) / 16 * 16;
-    // Up to 32 tokens by K pieces, more by pairs (4608 x 5120: 8.2 us against 9.0 with 1
-    // token, 9.4 against 9.1 with 32, 11.7 against 9.0 with 64).
+    // Up to 32 tokens by K pieces, more by pairs (4608 x 5120: 7.7 us against 10.5
+    // with 1 token, 9.0 against 9.6 with 32; 5120 x 2304: 6.1 against 7.0, 7.1 against 6.6).
     if (p.m > 32) return pair_launch(p, prefetch, sms, st);
     return p.m <= 16 ? split_launch<16>(p, prefetch, sms, st) : split_launch<32>(p, prefetch, sms, st);
   }

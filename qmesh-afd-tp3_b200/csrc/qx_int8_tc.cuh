@@ -183,7 +183,7 @@ __device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
 // others' sums instead needs a second cluster barrier before a CTA may leave, 1.5 us.)
 // With SwiGLU the 128 rows are 64 gate rows and their 64 up rows. The weights' bytes
 // bound it, and at a few us the launch: 4608 x 5120 for one token streams 23.6 MB in
-// 3.8 of the kernel's 7 us. The ring takes half an SM, so that two CTAs run side by side.
+// 3.8 of the kernel's 7.7 us. The ring takes half an SM, so that two CTAs run side by side.
 template <int BN>
 struct Split {
   static constexpr uint32_t A_BYTES = 128 * KST, STAGE = A_BYTES + BN * KST;
@@ -435,7 +435,8 @@ static_assert(PAIR_SMEM + 1536 <= 232448, "with the static part, one SM's memory
 // issues the MMAs of both (always M = 256: the rows from tb on read whatever follows
 // in shared memory and are not used). With SwiGLU the tile's weight rows are bn/2 gate
 // rows (CTA 0's copies) and their up rows (CTA 1's). The ring holds as many stages as
-// fit (6 of one span for tb = 128, bn = 256). Tiles of 512 tokens (every weight copy used twice, one
+// fit (6 of one span for tb = 128, bn = 256). Measured: 8192 x 5120 x 5120 160 us, the
+// power cap's rate; 8192 x 5120 x 2304 68 us (2.8 POP/s); 2048 x 5120 x 2304 20.6. Tiles of 512 tokens (every weight copy used twice, one
 // accumulator per block) were slower from 2048 tokens up: their epilogues run alone,
 // and all at once.
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)

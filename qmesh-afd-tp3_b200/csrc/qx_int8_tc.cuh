@@ -357,8 +357,10 @@ __device__ __forceinline__ bool epilogue_and(bool pred) {
 constexpr int PAIR_BLOCK = 32 * 64;
 
 // Up to 32 tokens (rows) x COLS output columns from column n on, each lane holding its
-// token's values. Rows on 16-byte boundaries (tma): one tiled store, which leaves out what
-// lies past the tensor's end; else element by element, 64 bytes of a row at a time.
+// token's values. Rows on 16-byte boundaries (tma): one tiled store, which leaves out rows
+// past the tensor's end, but writes its last columns in whole pieces of 16 bytes: a block
+// whose row ends inside such a piece, and rows on other boundaries, are stored element by
+// element, 64 bytes of a row at a time.
 template <int COLS>
 __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to, uint8_t* stage, int64_t row0, int rows,
                                             int n, const float* v, int tma, int lane) {
@@ -378,7 +380,7 @@ __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to
           make_uint4(pack2(p.type, v[8 * j], v[8 * j + 1]), pack2(p.type, v[8 * j + 2], v[8 * j + 3]),
                      pack2(p.type, v[8 * j + 4], v[8 * j + 5]), pack2(p.type, v[8 * j + 6], v[8 * j + 7]));
   }
-  if (tma) {
+  if (tma && (n + COLS <= p.n || p.n * OSZ % 16 == 0)) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) {
@@ -402,6 +404,8 @@ __device__ __forceinline__ void store_block(const Args& p, const CUtensorMap* to
     }
   }
   __syncwarp();
+  // An empty group stands for this block, so that the next wait still counts two buffers.
+  if (tma && lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // Epilogue warps: two per quarter of the accumulator's lanes.

@@ -367,3 +367,22 @@ def test_far_offsets(cuda_ready):
     out = torch.as_strided(torch.zeros(3 * stride, dtype=torch.bfloat16, device="cuda"), (3, 40), (stride, 1))
     int8_matmul(rows_of(4, 3, 160)[2], dsa, dw, dsw, out=out)
     close(out, want, D, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m", [3, 50, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_outputs_inside_aligned_rows(cuda_ready, m, dtype):
+    """Output rows on 16-byte boundaries whose last column lies inside a 16-byte piece:
+    the columns behind it are left as they were."""
+    from qmesh_b200.int8 import int8_matmul, int8_swiglu
+    k = 160
+    for n in (1, 2, 3, 7, 9, 31, 33, 63, 100, 129, 250, 1003):
+        width = (n + 63) // 64 * 64 + 64
+        _, _, da, dsa = rows_of(n, m, k)
+        _, _, dw, dsw = rows_of(n + 1, 2 * n, k, 0.02)
+        for call, w, s in ((int8_matmul, dw[:n], dsw[:n]), (int8_swiglu, dw, dsw)):
+            buf = torch.full((m + 1, width), 7.0, dtype=dtype, device="cuda")
+            call(da, dsa, w, s, out=buf[:m, :n])
+            assert torch.equal(buf[:m, :n], call(da, dsa, w, s, out_dtype=dtype))
+            buf[:m, :n] = 7.0
+            assert (buf == 7.0).all(), f"n={n}"

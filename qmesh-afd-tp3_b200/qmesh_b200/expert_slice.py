@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .arena import Arena
-from .combine import combine_ordered
+from .combine import check_out, combine_ordered
 from .int8 import Int8Expert
 from .trace import rng
 
@@ -220,11 +220,14 @@ def prefill_slice(arena: Arena, li: int, x: torch.Tensor, ids: torch.Tensor, tw:
     ordered combine's arithmetic, bf16(fp32(routed) + fp32(shared)), each part BF16."""
     if arena.layout != "tc":
         raise ValueError("the prefill slice needs a tensor-core layout arena")
-    if shared is not None and shared.k != _lib.HIDDEN:
-        raise ValueError(f"the shared expert's width is {shared.k}, the slice's {_lib.HIDDEN}")
     c0 = arena.a0 if c0 is None else c0
     c1 = arena.a1 if c1 is None else c1
     rows = x.shape[0]
+    if shared is not None:
+        if shared.k != _lib.HIDDEN:
+            raise ValueError(f"the shared expert's width is {shared.k}, the slice's {_lib.HIDDEN}")
+        if out is not None:                       # the routed part goes to a buffer of its own
+            check_out(out, rows, x.device)
     if out is None:
         out = torch.empty(rows, _lib.HIDDEN, dtype=torch.bfloat16, device=x.device)
     if workspace is None:

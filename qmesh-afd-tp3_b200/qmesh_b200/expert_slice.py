@@ -224,8 +224,12 @@ def prefill_slice(arena: Arena, li: int, x: torch.Tensor, ids: torch.Tensor, tw:
     c1 = arena.a1 if c1 is None else c1
     rows = x.shape[0]
     if shared is not None:
+        if not isinstance(shared, Int8Expert):
+            raise TypeError(f"the shared expert must be an Int8Expert, got {type(shared).__name__}")
         if shared.k != _lib.HIDDEN:
             raise ValueError(f"the shared expert's width is {shared.k}, the slice's {_lib.HIDDEN}")
+        if shared.dev != x.device:
+            raise ValueError(f"the shared expert is on {shared.dev}, x on {x.device}")
         if out is not None:                       # the routed part goes to a buffer of its own
             check_out(out, rows, x.device)
     if out is None:

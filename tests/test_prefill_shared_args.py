@@ -59,6 +59,22 @@ def test_prefill_with_shared_expert_takes_outputs(chunk):
         assert calls == ["prefill", (ROWS, HID)] and (out is None or got is out)
 
 
+def test_prefill_refuses_other_shared_experts(chunk):
+    """Only a W8A8 expert of the chunk's width and device can be the shared expert."""
+    from qmesh_b200.int8 import Int8Expert
+    call, args, ex, calls = chunk
+    for bad in (args[0].view(0), args[0], torch.nn.Identity()):
+        with pytest.raises(TypeError):
+            call(*args, shared=bad)
+    narrow = Int8Expert(torch.zeros(64, 128, dtype=torch.int8), torch.ones(64), torch.zeros(128, 32, dtype=torch.int8),
+                        torch.ones(128))
+    away = Int8Expert(*(t.to("meta") for t in (ex.w13, ex.w13_scale, ex.w2, ex.w2_scale)))
+    for bad in (narrow, away):
+        with pytest.raises(ValueError):
+            call(*args, shared=bad)
+    assert not calls
+
+
 @pytest.mark.parametrize("out_f32", [False, True])
 def test_combine_refuses_outputs(monkeypatch, out_f32):
     """The ordered combine itself: its C entry sees a pointer and a stride only."""

@@ -194,7 +194,11 @@ def device_status(device=None) -> int:
 class Int8Expert:
     """A dense SwiGLU expert in 8 bits: q = quant(x); h = swiglu(q . w13^T) in FP32;
     q2 = quant(h); y = q2 . w2^T. w13 int8 [2 inter, k] (gate rows, then up rows), w2
-    int8 [k, inter], one FP32 scale per row of each. One C call (qx_int8_expert)."""
+    int8 [k, inter], one FP32 scale per row of each. One C call (qx_int8_expert).
+
+    The weights are the tensors given: they are not copied, what is written into them in
+    place counts from the next call on, and they cannot be exchanged for others (make
+    another expert)."""
 
     def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
                  swiglu_limit: float = SWIGLU_LIMIT):
@@ -209,10 +213,17 @@ class Int8Expert:
         for name, t in (("w13_scale", w13_scale), ("w2", w2), ("w2_scale", w2_scale)):
             if t.device != self.dev:
                 raise ValueError(f"{name} is on {t.device}, not on {self.dev}")
-        self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
+        # Views of its own: the addresses below stay those of memory that this object holds,
+        # whatever becomes of the caller's tensor objects.
+        self._held = tuple(t.detach() for t in (w13, w13_scale, w2, w2_scale))
         self.weights = (w13.data_ptr(), w13_stride, w13_scale.data_ptr(), w2.data_ptr(), w2_stride, w2_scale.data_ptr())
         self.k, self.inter = w13.shape[1], w13.shape[0] // 2
         self.limit = float(max(swiglu_limit, 0.0))
+
+    w13 = property(lambda self: self._held[0].detach())
+    w13_scale = property(lambda self: self._held[1].detach())
+    w2 = property(lambda self: self._held[2].detach())
+    w2_scale = property(lambda self: self._held[3].detach())
 
     @classmethod
     def from_weights(cls, w13: torch.Tensor, w2: torch.Tensor, swiglu_limit: float = SWIGLU_LIMIT) -> "Int8Expert":

@@ -65,6 +65,8 @@ def _slice_args(x, ids, tw, out, c0, c1, workspace, x_scale, swiglu_limit, has_l
         fmt = _lib.QX_X_E4M3 if x_scale.numel() == rows else _lib.QX_X_E4M3_POST
         if x_scale.numel() not in (1, rows):
             raise ValueError(f"x_scale has {x_scale.numel()} values for {rows} rows")
+        if not x_scale.is_contiguous():
+            raise ValueError(f"x_scale must be contiguous, got strides {x_scale.stride()}")
         esz = 1
     else:
         raise TypeError(f"x must be bf16 or e4m3, got {x.dtype}")

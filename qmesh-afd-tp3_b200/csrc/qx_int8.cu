@@ -344,6 +344,13 @@ uint64_t wait_limit_ns() {
   return (uint64_t)(ms < 10 ? 10 : ms) * 1000000ull;
 }
 
+// Test hook QX_TEST_INT8_HOLD=1: the few-token kernel's sums are waited for once more
+// than they are announced, so that the wait runs out and QX_DEV_TIMEOUT is recorded.
+int test_hold() {
+  const char* e = getenv("QX_TEST_INT8_HOLD");
+  return e ? atoi(e) : 0;
+}
+
 int element_size(int type) { return type == QX_T_F32 ? 4 : type == QX_T_E4M3 ? 1 : 2; }
 
 // Tiled-copy descriptor of rows x cols elements of 1, 2 or 4 bytes; places outside
@@ -456,7 +463,7 @@ int split_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
   if (!row_map(&tw, p.w, p.swiglu ? 2ll * p.n : p.n, p.k, p.ws, half) || !row_map(&ta, p.a, p.m, p.k, p.as, BN))
     return QX_ERR_DEVICE;
   return Launch(dim3((unsigned)(tiles * pieces), 1, 1), SPLIT_THR, L::SMEM, st, pieces)(
-      split_kernel<BN>, tw, ta, p, pieces, prefetch, wait_limit_ns());
+      split_kernel<BN>, tw, ta, p, pieces, prefetch, wait_limit_ns(), test_hold());
 }
 
 // A checked product. prefetch: the weights are complete when this kernel starts,

@@ -197,7 +197,7 @@ constexpr int SPLIT_THR = 224;
 template <int BN>
 __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant__ CUtensorMap tw,
                                                           const __grid_constant__ CUtensorMap ta, Args p, int pieces,
-                                                          int prefetch, uint64_t timeout) {
+                                                          int prefetch, uint64_t timeout, int hold) {
   using L = Split<BN>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[L::NS], empty[L::NS], done;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&done, 1);
+    mbar_init(&done, hold == 1 ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   const bool epi = warp >= 2 && warp < 6;
   pdl_wait();                                             // also: the tokens' scales, and the output's place
   if (epi) ok = wait_phase(&done, 0, 2 * timeout);
+  __syncwarp();                                           // a warp's lanes may have polled a different number of times
   cluster_wait();                                         // every CTA of the cluster has started
   if (epi && __all_sync(0xffffffffu, ok)) {
     tc::fence_after_sync();

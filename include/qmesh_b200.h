@@ -347,7 +347,7 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  *
  * qx_int8_status: the QX_DEV_* bits (QX_DEV_NONFINITE, QX_DEV_TIMEOUT) that these
  * calls recorded on the current device since the last read; reads, clears and
- * waits for `stream`. */
+ * waits for `stream`. A call that met QX_DEV_TIMEOUT leaves its outputs undefined. */
 #define QX_INT8_MAX_K 131071
 
 typedef struct {

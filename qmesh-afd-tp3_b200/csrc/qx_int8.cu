@@ -344,8 +344,10 @@ uint64_t wait_limit_ns() {
   return (uint64_t)(ms < 10 ? 10 : ms) * 1000000ull;
 }
 
-// Test hook QX_TEST_INT8_HOLD=1: the few-token kernel's sums are waited for once more
-// than they are announced, so that the wait runs out and QX_DEV_TIMEOUT is recorded.
+// Test hook QX_TEST_INT8_HOLD: bounded waits that run out, with QX_DEV_TIMEOUT recorded. 1:
+// the barriers behind which the epilogues read the sums expect one arrival too many; 2: the
+// thread that issues the MMAs waits for something that does not come before it takes the
+// first stage, and gives up with a ring full of copies in flight.
 int test_hold() {
   const char* e = getenv("QX_TEST_INT8_HOLD");
   return e ? atoi(e) : 0;
@@ -441,7 +443,7 @@ int pair_launch(const Args& p, int prefetch, int sms, cudaStream_t st) {
   const int tma = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.os * osz % 16 == 0 &&
                   tiled_map(&to, p.out, osz, p.m, p.n, p.os * osz, 64 / osz, 32, CU_TENSOR_MAP_SWIZZLE_64B);
   return Launch(dim3(2 * pairs, 1, 1), PAIR_THR, PAIR_SMEM, st, 2)(pair_kernel, tw, ta, to, p, tb, bn, spans, tiles_m,
-                                                                  (int)tiles, prefetch, tma, wait_limit_ns());
+                                                                  (int)tiles, prefetch, tma, wait_limit_ns(), test_hold());
 }
 
 // K pieces of the split kernel (1..8): the fewest that leave a CTA the least of K while

@@ -141,6 +141,34 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint6
   return try_phase(bar, parity) || wait_long(bar, parity, limit);
 }
 
+// Bytes that stand for copies which were never issued.
+__device__ __forceinline__ void complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// After the MMA thread has given up: waits (each bounded) until the copies in flight have
+// landed, so that none writes into shared memory after the CTAs have left. A stage's fill
+// is brought in by N copy threads, thread i having issued its `bytes[i]` of the first
+// issued[i] fills; thread 0 also announces the bytes of them all. No thread is more than
+// one round of the ring ahead of the MMAs, so the last ns fills are in ns different stages.
+// A fill that only some threads have issued is made to complete with those: the bytes
+// of the others are counted as if they had come, or, where thread 0 is behind, the bytes
+// that are under way are announced in its place.
+template <int N>
+__device__ __noinline__ void drain_copies(uint64_t* full, uint32_t ns, const uint32_t* issued, const uint32_t (&bytes)[N],
+                                          uint64_t timeout) {
+  uint32_t last = 0;
+  for (int i = 0; i < N; ++i) last = max(last, issued[i]);
+  for (uint32_t f = last > ns ? last - ns : 0u; f < last; ++f) {
+    uint32_t in = 0, out = 0;
+    for (int i = 0; i < N; ++i) (f < issued[i] ? in : out) += bytes[i];
+    uint64_t* bar = &full[f % ns];
+    if (f >= issued[0]) mbar_arrive_expect_tx(bar, in);
+    else if (out) complete_tx(bar, out);
+    wait_phase(bar, (f / ns) & 1, timeout);
+  }
+}
+
 // ---- accumulator loads ---------------------------------------------------------------
 __device__ __forceinline__ void tm_ld32(uint32_t taddr, int32_t (&r)[32]) {
   asm volatile(
@@ -201,7 +229,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   using L = Split<BN>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[L::NS], empty[L::NS], done;
-  __shared__ uint32_t tmem;
+  __shared__ uint32_t tmem, gave_up, issued[2];          // issued: fills whose weights, tokens were sent for
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const uint32_t sums = smem_u32(ring) + L::NS * L::STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -221,6 +249,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, hold == 1 ? 2 : 1);
+    gave_up = issued[0] = issued[1] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -232,6 +261,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   __syncthreads();
   tc::fence_after_sync();
   bool ok = true;
+  uint32_t fills = 0;                                     // of a copy thread: stages it has sent for
   if (warp == 0 && elect_one()) {
     if (!prefetch) pdl_wait();
     const uint32_t base = smem_u32(ring), bars = smem_u32(full);
@@ -243,10 +273,8 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       mbar_arrive_expect_tx(&full[s], L::STAGE);
       tma_2d(base + s * L::STAGE, &tw, c * (int)KST, n0, bars + 8 * s);
       if (p.swiglu) tma_2d(base + s * L::STAGE + 64 * KST, &tw, c * (int)KST, p.n + n0, bars + 8 * s);
+      ++fills;
       if (++s == L::NS) s = 0, ph ^= 1;
-    }
-    if (!ok) {                                            // copies still in flight land before the CTA leaves
-      for (int i = 0; i < L::NS; ++i) wait_phase(&full[i], 0, timeout);
     }
   } else if (warp == 6 && elect_one()) {
     pdl_wait();
@@ -256,13 +284,15 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
     for (int c = c0; c < c1; ++c) {
       if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
       tma_2d(base + s * L::STAGE, &ta, c * (int)KST, 0, bars + 8 * s);
+      ++fills;
       if (++s == L::NS) s = 0, ph ^= 1;
     }
   } else if (warp == 1 && elect_one()) {
     pdl_wait();
     int s = 0;
     uint32_t ph = 0;
-    for (int c = c0; c < c1; ++c) {
+    if (hold == 2) ok = wait_phase(&done, 0, timeout);
+    for (int c = c0; ok && c < c1; ++c) {
       if (!(ok = wait_phase(&full[s], ph, timeout))) break;
       tc::fence_after_sync();
       const uint64_t da = sdesc128(smem_u32(ring) + s * L::STAGE), db = da + (L::A_BYTES >> 4);
@@ -271,6 +301,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
       tc::commit(&empty[s]);
       if (++s == L::NS) s = 0, ph ^= 1;
     }
+    if (!ok) gave_up = 1;
     tc::commit(&done);
   }
   __syncwarp();
@@ -300,6 +331,11 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   }
   cluster_sync();
   if (warp == 1) tc::tmem_dealloc(tmem, L::COLS);
+  if (gave_up) {                                          // copies may still be in flight to this CTA
+    if (fills) issued[warp == 0 ? 0 : 1] = fills;
+    __syncthreads();
+    if (threadIdx.x == 0) drain_copies<2>(full, L::NS, issued, {L::A_BYTES, L::STAGE - L::A_BYTES}, timeout);
+  }
   // items of this CTA: (own token, four weight rows)
   const int per = half / 4, items = (p.m - rank + pieces - 1) / pieces * per;
   const int four = p.type == QX_T_F32 ? 16 : 8;           // bytes of four outputs
@@ -447,10 +483,10 @@ static_assert(PAIR_SMEM + 1536 <= 232448, "with the static part, one SM's memory
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap ta,
                 const __grid_constant__ CUtensorMap to, Args p, int tb, int bn, int spans, int tiles_m, int tiles,
-                int prefetch, int tma, uint64_t timeout) {
+                int prefetch, int tma, uint64_t timeout, int hold) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[MAX_NS], empty[MAX_NS], acc_full[2], acc_empty[2], drained;
-  __shared__ uint32_t tmem;
+  __shared__ uint32_t tmem, gave_up, issued[4];          // issued: as in the other kernel, by CTA 0's copies, then CTA 1's
   __shared__ __align__(16) float sws[256];              // the tile's weight scales
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -472,10 +508,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_full[b], hold == 1 ? 2 : 1);
       mbar_init(&acc_empty[b], 2 * PAIR_EPI);
     }
     mbar_init(&drained, 1);
+    gave_up = issued[0] = issued[1] = issued[2] = issued[3] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -488,6 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   cluster_sync();
   tc::fence_after_sync();
   bool ok = true;
+  uint32_t fills = 0;                                     // of a copy thread: stages it has sent for
   if (warp == 0 && elect_one()) {
     const uint32_t bytes = 2 * stage_bytes;               // both CTAs' copies
     // Weights (and CTA 0's count of both CTAs' bytes of a stage). Weights that are
@@ -505,13 +543,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
         if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
         for (int g = 0; g < spans; ++g)
           tma_2d_pair(base + s * stage_bytes + g * b_span, &tw, c * kst + g * (int)KST, n0, bars + 8 * s);
+        ++fills;
         if (++s == ns) s = 0, ph ^= 1;
       }
-    }
-    // Copies still in flight after a wait that ran out count on CTA 0's barriers;
-    // the cluster barrier below holds CTA 1 until CTA 0 has waited for them.
-    if (!ok && rank == 0) {
-      for (int i = 0; i < ns; ++i) wait_phase(&full[i], 0, timeout);
     }
   } else if (warp == 2 + PAIR_EPI && elect_one()) {
     pdl_wait();
@@ -524,6 +558,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
         if (!(ok = wait_phase(&empty[s], ph, timeout))) break;
         for (int g = 0; g < spans; ++g)
           tma_2d_pair(base + s * stage_bytes + g * a_span, &ta, c * kst + g * (int)KST, m0, bars + 8 * s);
+        ++fills;
         if (++s == ns) s = 0, ph ^= 1;
       }
     }
@@ -532,6 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     pdl_wait();
     int s = 0, it = 0;
     uint32_t ph = 0;
+    if (hold == 2) ok = wait_phase(&drained, 0, timeout);
     for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
       const int b = it & 1;
       if (!(ok = wait_phase(&acc_empty[b], ((it >> 1) & 1) ^ 1, timeout))) break;
@@ -549,7 +585,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
         commit_pair(&empty[s]);
         if (++s == ns) s = 0, ph ^= 1;
       }
-      commit_pair(&acc_full[b]);
+      if (ok) commit_pair(&acc_full[b]);                  // else the tile's outputs are not written
+    }
+    if (!ok) {                                            // seen in both CTAs behind the cluster barrier below
+      for (uint32_t r = 0; r < 2; ++r) st_cluster(mapa(smem_u32(&gave_up), r), 1);
+      asm volatile("fence.acq_rel.cluster;" ::: "memory");
     }
     commit_pair(&drained);
     wait_phase(&drained, 0, 2 * timeout);          // no MMA is in flight when TMEM is released
@@ -627,6 +667,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
   tc::fence_before_sync();
   cluster_arrive_relaxed();
   cluster_wait();
+  if (gave_up) {
+    // Copies may still be in flight to either CTA; all of them count on CTA 0's barriers,
+    // which waits for them, and neither CTA leaves before.
+    if (fills) st_cluster(mapa(smem_u32(&issued[2 * rank + (warp == 0 ? 0 : 1)]), 0), (int32_t)fills);
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0 && threadIdx.x == 0) {
+      const uint32_t w = spans * b_span, t = spans * a_span;
+      drain_copies<4>(full, ns, issued, {w, t, w, t}, timeout);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

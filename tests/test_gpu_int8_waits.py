@@ -37,3 +37,18 @@ def check(monkeypatch, hold, m, n, k):
 @pytest.mark.parametrize("m,n,k", [(1, 4608, 5120), (16, 130, 96), (32, 2304, 640)])
 def test_few_token_kernel_sums_never_come(cuda_ready, monkeypatch, m, n, k):
     check(monkeypatch, 1, m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 2000), (100, 64, 96), (2048, 5120, 2304)])
+def test_pair_kernel_sums_never_come(cuda_ready, monkeypatch, m, n, k):
+    """With three tiles per pair of CTAs the MMAs come to a stop too, in the middle of a
+    ring of copies."""
+    check(monkeypatch, 1, m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4608, 5120), (16, 130, 96), (32, 2304, 640), (3, 64, 20000),
+                                   (40, 300, 2000), (100, 64, 96), (2048, 5120, 2304)])
+def test_copies_in_flight_when_the_mmas_give_up(cuda_ready, monkeypatch, m, n, k):
+    """Short rings and full ones: what was sent for lands before the CTA leaves, so the next
+    call finds its shared memory to itself."""
+    check(monkeypatch, 2, m, n, k)

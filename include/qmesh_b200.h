@@ -346,8 +346,10 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  * nothing; out must not overlap the inputs.
  *
  * qx_int8_status: the QX_DEV_* bits (QX_DEV_NONFINITE, QX_DEV_TIMEOUT) that these
- * calls recorded on the current device since the last read; reads, clears and
- * waits for `stream`. A call that met QX_DEV_TIMEOUT leaves its outputs undefined. */
+ * calls recorded on the current device since the last read: one word for all
+ * streams and callers of the device, so a read takes the reports of all of them. It
+ * is read and cleared in one step (a bit set meanwhile is in this read or the next)
+ * and the call waits for `stream`. A call that met QX_DEV_TIMEOUT leaves its outputs undefined. */
 #define QX_INT8_MAX_K 131071
 
 typedef struct {

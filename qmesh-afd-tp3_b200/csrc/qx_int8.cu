@@ -16,6 +16,9 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <atomic>
+#include <thread>
+
 #include "qmesh_b200.h"
 #include "qx_ptx.cuh"
 
@@ -28,6 +31,12 @@ constexpr uint32_t INF_BITS = 0x7f800000u;
 
 // QX_DEV_* bits of this file's kernels since the last qx_int8_status.
 __device__ uint32_t g_status;
+
+// Read and cleared in one step, so that no bit set beside a read is lost, into a word
+// that belongs to the read until it returns.
+constexpr int STATUS_READS = 64;
+__device__ uint32_t g_taken[STATUS_READS];
+__global__ void take_status_kernel(int slot) { g_taken[slot] = atomicExch(&g_status, 0u); }
 
 // ------------------------------------------------------------------ outputs
 __device__ __forceinline__ void store_out(void* out, int64_t i, int type, float v) {
@@ -626,13 +635,22 @@ int qx_int8_expert(const QxInt8ExpertArgs* a, void* stream) {
 
 int qx_int8_status(uint32_t* status, void* stream) {
   if (!status) return QX_ERR_ARG;
-  void* addr = nullptr;
-  if (cudaGetSymbolAddress(&addr, g_status) != cudaSuccess) return QX_ERR_DEVICE;
+  if (device_sms() <= 0) return QX_ERR_DEVICE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (cudaMemcpyAsync(status, addr, sizeof(uint32_t), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
-      cudaMemsetAsync(addr, 0, sizeof(uint32_t), st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess)
-    return QX_ERR_LAUNCH;
-  return QX_OK;
+  static std::atomic<uint64_t> busy{0};                   // words of g_taken in use
+  uint64_t b = busy.load();
+  int slot = 0;
+  do {
+    while (b == ~0ull) std::this_thread::yield(), b = busy.load();
+    slot = __builtin_ctzll(~b);
+  } while (!busy.compare_exchange_weak(b, b | 1ull << slot));
+  take_status_kernel<<<1, 1, 0, st>>>(slot);
+  bool ok = cudaGetLastError() == cudaSuccess;
+  ok = ok && cudaMemcpyFromSymbolAsync(status, g_taken, sizeof(uint32_t), slot * sizeof(uint32_t), cudaMemcpyDeviceToHost,
+                                       st) == cudaSuccess;
+  ok = cudaStreamSynchronize(st) == cudaSuccess && ok;
+  busy.fetch_and(~(1ull << slot));
+  return ok ? QX_OK : QX_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -182,7 +182,8 @@ def int8_swiglu(q: torch.Tensor, scale: torch.Tensor, w13: torch.Tensor, w13_sca
 
 def device_status(device=None) -> int:
     """QX_DEV_* bits (NONFINITE, TIMEOUT) that this module's calls recorded on `device`
-    (default: the current one) since the last read (synchronises and clears)."""
+    (default: the current one) since the last read: one word for all streams and callers of
+    the device, read and cleared in one step (synchronises the current stream)."""
     dev = torch.device("cuda" if device is None else device)
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())

@@ -340,7 +340,7 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  * w holds n gate rows and then n up rows (w_scale too) and out[i, j] =
  * g / (1 + exp(-g)) * u, with g = min(g, limit) and u = clamp(u, -limit, limit)
  * first if has_limit (the quotient to 2 units of its last
- * place, and 0 for g below -87.3). Strides in elements. The same bytes come out whatever m and
+ * place, and 0 for g below -88.7, where exp(-g) is past FP32). Strides in elements. The same bytes come out whatever m and
  * the alignment are; rows of a and w that start on 16-byte boundaries (address
  * and stride) run on the tensor cores, others on a slower path. m = 0 does
  * nothing; out must not overlap the inputs.

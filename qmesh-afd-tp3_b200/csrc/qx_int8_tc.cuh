@@ -148,20 +148,20 @@ __device__ __forceinline__ void complete_tx(uint64_t* bar, uint32_t bytes) {
 
 // After the MMA thread has given up: waits (each bounded) until the copies in flight have
 // landed, so that none writes into shared memory after the CTAs have left. A stage's fill
-// is brought in by N copy threads, thread i having issued its `bytes[i]` of the first
-// issued[i] fills; thread 0 also announces the bytes of them all. No thread is more than
+// is brought in by n copy threads, weights and tokens in turn, thread i having issued its
+// `wb` or `tb` bytes of the first issued[i] fills; thread 0 also announces the bytes of them
+// all. No thread is more than
 // one round of the ring ahead of the MMAs, so the last ns fills are in ns different stages.
 // A fill that only some threads have issued is made to complete with those: the bytes
 // of the others are counted as if they had come, or, where thread 0 is behind, the bytes
 // that are under way are announced in its place.
-template <int N>
-__device__ __noinline__ void drain_copies(uint64_t* full, uint32_t ns, const uint32_t* issued, const uint32_t (&bytes)[N],
-                                          uint64_t timeout) {
+__device__ __noinline__ void drain_copies(uint64_t* full, uint32_t ns, const uint32_t* issued, int n, uint32_t wb,
+                                          uint32_t tb, uint64_t timeout) {
   uint32_t last = 0;
-  for (int i = 0; i < N; ++i) last = max(last, issued[i]);
+  for (int i = 0; i < n; ++i) last = max(last, issued[i]);
   for (uint32_t f = last > ns ? last - ns : 0u; f < last; ++f) {
     uint32_t in = 0, out = 0;
-    for (int i = 0; i < N; ++i) (f < issued[i] ? in : out) += bytes[i];
+    for (int i = 0; i < n; ++i) (f < issued[i] ? in : out) += i & 1 ? tb : wb;
     uint64_t* bar = &full[f % ns];
     if (f >= issued[0]) mbar_arrive_expect_tx(bar, in);
     else if (out) complete_tx(bar, out);
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(SPLIT_THR) split_kernel(const __grid_constant_
   if (gave_up) {                                          // copies may still be in flight to this CTA
     if (fills) issued[warp == 0 ? 0 : 1] = fills;
     __syncthreads();
-    if (threadIdx.x == 0) drain_copies<2>(full, L::NS, issued, {L::A_BYTES, L::STAGE - L::A_BYTES}, timeout);
+    if (threadIdx.x == 0) drain_copies(full, L::NS, issued, 2, L::A_BYTES, L::STAGE - L::A_BYTES, timeout);
   }
   // items of this CTA: (own token, four weight rows)
   const int per = half / 4, items = (p.m - rank + pieces - 1) / pieces * per;
@@ -673,10 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THR, 1)
     if (fills) st_cluster(mapa(smem_u32(&issued[2 * rank + (warp == 0 ? 0 : 1)]), 0), (int32_t)fills);
     __syncwarp();
     cluster_sync();
-    if (rank == 0 && threadIdx.x == 0) {
-      const uint32_t w = spans * b_span, t = spans * a_span;
-      drain_copies<4>(full, ns, issued, {w, t, w, t}, timeout);
-    }
+    if (rank == 0 && threadIdx.x == 0) drain_copies(full, ns, issued, 4, spans * b_span, spans * a_span, timeout);
     __syncwarp();
     cluster_sync();
   }

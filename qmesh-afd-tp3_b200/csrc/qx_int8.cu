@@ -500,9 +500,15 @@ int product(Args p, int prefetch, int sms, cudaStream_t st) {
     return p.m <= 16 ? split_launch<16>(p, prefetch, sms, st) : split_launch<32>(p, prefetch, sms, st);
   }
   const int half = p.swiglu ? ST / 2 : ST;
-  const int64_t gy = (p.m + ST - 1) / ST;
-  if (gy > 65535) return QX_ERR_SHAPE;
-  return Launch(dim3((unsigned)((p.n + half - 1) / half), (unsigned)gy, 1), 256, 0, st)(plain_kernel, p);
+  int rc = QX_OK;
+  for (int64_t left = p.m; rc == QX_OK && left > 0; left -= p.m) {   // row blocks of what a grid's y counts
+    p.m = (int)(left < 65535ll * ST ? left : 65535ll * ST);
+    rc = Launch(dim3((unsigned)((p.n + half - 1) / half), (unsigned)((p.m + ST - 1) / ST), 1), 256, 0, st)(plain_kernel, p);
+    p.a += p.m * p.as;
+    p.sa += p.m;
+    p.out = reinterpret_cast<uint8_t*>(p.out) + p.m * p.os * element_size(p.type);
+  }
+  return rc;
 }
 
 template <int T>

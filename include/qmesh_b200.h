@@ -301,8 +301,8 @@ int qx_slice_decode_tc_shared(const QxArena* arena, const QxSliceArgs* args, con
  * qx_slice_decode_tc, except that ids, ids_int64 and tw are not read and the
  * workspace has qx_moe_workspace_bytes bytes (0 for sizes the call refuses:
  * 1..QX_MAX_ROWS rows, topk 1..min(QX_MAX_TOPK, n_experts), n_experts up to 4096).
- * A row whose logits hold a NaN or +infinity has NaN weights and a NaN output;
- * the other rows are as without it. Capture-safe; calls that may overlap on the
+ * A row of x that holds a NaN or an infinity, or whose logits do (a NaN or +infinity),
+ * has NaN weights and a NaN output; the other rows are as without it. Capture-safe; calls that may overlap on the
  * GPU need a workspace each. */
 typedef struct {
   const void*  gate;         /* router weights [n_experts, 5120], 16-byte aligned rows */

@@ -196,6 +196,23 @@ __device__ void select_row(const float* l, size_t step, int E, int topk, int lan
   w_out = my_id >= 0 ? w / sum : 0.f;
 }
 
+// Whether row r of the activations holds a NaN or an infinity (a whole warp asks). Only
+// rows for which nothing was selected need it: an infinity times router weights of one
+// sign makes every logit -infinity, as masks of all experts do.
+__device__ __forceinline__ bool row_nonfinite(const Params& p, int r, int lane) {
+  const float inv = p.x_fmt == QX_X_E4M3 ? p.x_scale[r] : p.x_fmt == QX_X_E4M3_POST ? p.x_scale[0] : 1.f;
+  const uint8_t* xr = reinterpret_cast<const uint8_t*>(p.x) + (size_t)r * p.x_stride;
+  bool bad = false;
+#pragma unroll 1
+  for (int k = 8 * lane; k < HID; k += 256) {
+    const uint4 v = load_x8(p, xr, k, inv);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  }
+  return __any_sync(0xffffffffu, bad);
+}
+
 // ------------------------------------------------------------------ kernels in front
 // CTAs: one per (8 experts, 16 rows, quarter of K).
 template <int GT>
@@ -229,6 +246,10 @@ __global__ void __launch_bounds__(PREP_THR) moe_prep_kernel(Params p, int nsel) 
   int id;
   float w;
   select_row(p.logits + (size_t)r * E4, (size_t)p.rows * E4, p.E, p.topk, lane, keys + warp * E4, id, w);
+  if (__shfl_sync(0xffffffffu, id, 0) < 0 && row_nonfinite(p, r, lane)) {   // a NaN row, as if its logits were NaN
+    id = lane;
+    w = __uint_as_float(0x7fc00000u);
+  }
   if (lane < p.topk) {
     const int q = r * p.topk + lane;
     p.sel_ids[q] = id;

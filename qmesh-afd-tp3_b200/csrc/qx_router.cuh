@@ -10,9 +10,13 @@
 // CTA over all of K, four rounds of loads, took 9 us with one row). A lane reads 8
 // consecutive elements of its row and of its expert, which are the operands of two
 // products under one and the same permutation of K. Products of BF16 values are exact;
-// FP32 router weights enter as three BF16 parts, w = hi + mid + lo to 2^-26. Each
-// block's sum starts from zero and is added in FP32, so that a logit's error stays near
-// 2^-24 of its partial sums; the quarters' sums are added where the logits are read.
+// FP32 router weights enter as three BF16 parts, w = hi + mid + lo exactly (24 bits are
+// three times 8). What PTX promises of the sums inside a product is single precision in
+// an unspecified order and rounding, 2^-23 an addition: each block's 32 products start from
+// zero, and the blocks, warps, quarters and the bias are added in FP32 (16 additions), so a
+// logit is within (2 * 32 + 16) 2^-24 of its sum |x w| (a little over one more for FP32
+// weights, whose smaller parts are added first). The quarters' sums are added where the logits
+// are read.
 constexpr int RE = 8, RR = 16, RWARPS = PREP_THR / 32, RSPLIT = 4, RK = HID / RSPLIT / RWARPS, RB = RK / 32;
 static_assert(RK % 32 == 0, "whole blocks of K per warp");
 

@@ -343,7 +343,7 @@ int qx_moe_decode_tc(const QxArena* arena, const QxSliceArgs* args, const QxRout
  * place, and 0 for g below -88.7, where exp(-g) is past FP32). Strides in elements. The same bytes come out whatever m and
  * the alignment are; rows of a and w that start on 16-byte boundaries (address
  * and stride) run on the tensor cores, others on a slower path. m = 0 does
- * nothing; out must not overlap the inputs.
+ * nothing, m and n go up to 2^24; out must not overlap the inputs.
  *
  * qx_int8_status: the QX_DEV_* bits (QX_DEV_NONFINITE, QX_DEV_TIMEOUT) that these
  * calls recorded on the current device since the last read: one word for all

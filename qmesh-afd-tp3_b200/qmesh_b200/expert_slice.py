@@ -11,9 +11,9 @@ layout arena, qx_slice_decode for a register-dequant layout arena):
   with the signature, argument meaning and errors of gx/gx_decode_swz.py:148-179
   (x is the ingested BF16 activation; out is written in place).
 
-Everything is launched on the current torch stream, allocates nothing once the
-workspace exists, and never synchronises the host, so both forms can be captured
-in a CUDA graph.
+Both forms are launched on the current torch stream, allocate nothing once the
+workspace exists, and never synchronise the host, so they can be captured in a CUDA
+graph.
 """
 
 from __future__ import annotations
@@ -219,7 +219,9 @@ def prefill_slice(arena: Arena, li: int, x: torch.Tensor, ids: torch.Tensor, tw:
                   swiglu_limit: float = SWIGLU_LIMIT, shared: Int8Expert | None = None) -> torch.Tensor:
     """BF16 [rows, 5120] partial of a prefill chunk over columns [c0, c1) (W4A4). With
     `shared`, a W8A8 expert over the same rows is added after the routed partial in the
-    ordered combine's arithmetic, bf16(fp32(routed) + fp32(shared)), each part BF16."""
+    ordered combine's arithmetic, bf16(fp32(routed) + fp32(shared)), each part BF16. The
+    expert has its own SwiGLU limit from its construction; both parts and its workspace are
+    allocated per call, its reports go to `int8.device_status`."""
     if arena.layout != "tc":
         raise ValueError("the prefill slice needs a tensor-core layout arena")
     c0 = arena.a0 if c0 is None else c0

@@ -42,7 +42,10 @@ def moe_layer(arena: Arena, li: int, x: torch.Tensor, gate: torch.Tensor, bias: 
               workspace: torch.Tensor | None = None, swiglu_limit: float = SWIGLU_LIMIT) -> torch.Tensor:
     """BF16 [rows, 5120] = sum over the topk experts of x . gate^T (+ bias) of their
     softmax weight (over the selected) times the expert over columns [c0, c1), plus
-    the shared expert: the view of a one-expert tensor-core arena, or an `Int8Expert`.
+    the shared expert: the view of a one-expert tensor-core arena, which `swiglu_limit`
+    clamps too, or an `Int8Expert`, which has its own limit from its construction (its
+    FP32 output and its workspace are allocated per call, its reports go to
+    `int8.device_status`).
     All parts are summed in FP32 and rounded once. `ids` (int32 [rows, topk]) and `tw`
     (float32) receive the selection when given. 1 to 64 rows."""
     if arena.layout != "tc":

@@ -149,12 +149,11 @@ __device__ __forceinline__ void complete_tx(uint64_t* bar, uint32_t bytes) {
 // After the MMA thread has given up: waits (each bounded) until the copies in flight have
 // landed, so that none writes into shared memory after the CTAs have left. A stage's fill
 // is brought in by n copy threads, weights and tokens in turn, thread i having issued its
-// `wb` or `tb` bytes of the first issued[i] fills; thread 0 also announces the bytes of them
-// all. No thread is more than
-// one round of the ring ahead of the MMAs, so the last ns fills are in ns different stages.
-// A fill that only some threads have issued is made to complete with those: the bytes
-// of the others are counted as if they had come, or, where thread 0 is behind, the bytes
-// that are under way are announced in its place.
+// `wb` or `tb` bytes of the first issued[i] fills; thread 0 also announces the bytes of all.
+// No thread is more than one round of the ring ahead of the MMAs, so the last ns fills are
+// in ns different stages. A fill that only some threads have issued is made to complete with
+// those: the bytes of the others are counted as if they had come, or, where thread 0 is
+// behind, the bytes that are under way are announced in its place.
 __device__ __noinline__ void drain_copies(uint64_t* full, uint32_t ns, const uint32_t* issued, int n, uint32_t wb,
                                           uint32_t tb, uint64_t timeout) {
   uint32_t last = 0;
